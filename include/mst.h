@@ -27,6 +27,10 @@
  *                            model/train.py:132-135,140,158     nn.L1Loss fwd/bwd, nn.MSELoss (test)
  *   mst_adam_f32 / _ex_f32 / _dev_f32
  *                            model/train.py:188,143             optim.Adam(lr=1e-3)
+ *   mst_grad_norm, mst_grad_scale, mst_adam_clip_f32
+ *                            (none: beside optim.Adam)           gradient norm, clipping, clipped Adam
+ *   mst_gated_fwd / _bwd / _step
+ *                            (none: beside the NCL layers)       gated linear recurrence over time
  *   mst_onoff_f32            preprocessing/preprocess.py:148-155 piano-roll binarise + onset/offset
  *   mst_render_logpow_f32 / _bwd_f32
  *                            model/inference.py:109 sqrt(expm1(clip(S,0,20))) with a held phase:
@@ -48,6 +52,11 @@ extern "C" {
 #define MST_ACT_NONE 0
 #define MST_ACT_RELU 1
 #define MST_ACT_LRELU 2
+
+/* element types of the entry points that take one */
+#define MST_F32 0
+#define MST_BF16 1
+#define MST_F16 2
 
 #define MST_PAD_REFLECT 0
 #define MST_PAD_CONSTANT 1
@@ -193,6 +202,49 @@ int mst_adam_ex_f32(float* p, const float* g, float* m, float* v, int64_t n, flo
  * on the device from its own step counter, so one recorded launch serves every step. */
 int mst_adam_dev_f32(float* p, const float* g, float* m, float* v, int64_t n, const float* hyper,
                      float b2, float one_minus_b1, float one_minus_b2, float eps, void* stream);
+
+/* ---- global gradient norm and clipping, over `count` tensors of any of the element types ----
+ * grads[i]: device pointer, aligned to its elements, numel[i] >= 0 elements in any order (a dense
+ * tensor's memory); grads, numel and types are HOST arrays, read before the call returns.
+ *   norm[0] = sqrt(sum of g^2 over every element)  (sums in double, in one fixed order)
+ * scale: g *= min(1, max_norm / (norm[0] + 1e-6)) in place (max_norm >= 0), the product in float,
+ * rounded once to the element type. A norm that is not a number makes the factor one. Ranges that
+ * are written must not overlap (MST_EINVAL). */
+size_t mst_grad_norm_workspace_size(int32_t count);
+int mst_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* types, int32_t count,
+                  float* norm, void* workspace, size_t ws_bytes, void* stream);
+int mst_grad_scale(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count,
+                   const float* norm, float max_norm, void* stream);
+/* mst_adam_f32's update over `count` tensors (HOST arrays of device pointers), each gradient taken
+ * times min(1, max_norm / (norm[0] + 1e-6)); the gradients stay as they are. hyper (nullable) as in
+ * mst_adam_dev_f32. The elements of p, g, m, v of one tensor are in one order; 4-byte alignment. */
+int mst_adam_clip_f32(float* const* p, const float* const* g, float* const* m, float* const* v,
+                      const int64_t* numel, int32_t count, const float* norm, float max_norm,
+                      float lr_step, float b2, float one_minus_b1, float one_minus_b2, float eps,
+                      float bc2_sqrt, const float* hyper, void* stream);
+
+/* ---- gated linear recurrence over time, element type `type` (MST_F32 / MST_BF16 / MST_F16) ----
+ *   a_t = sigmoid(gate_t);  h_t = a_t h_{t-1} + (1 - a_t) x_t,  h_{-1} = h0 (nullable: zeros)
+ * x, gate: (B, C, T) by batch and channel strides (elements), unit time stride. lengths (nullable,
+ * B on the device, taken into [0, T]): frames at or past lengths[b] are not read, leave the state
+ * as it is and give h = 0. reverse != 0: t runs from the last frame down, h0 enters there.
+ * h: (B, C, T) contiguous; last (B, C): the state after the last frame (the first when reversed).
+ * carry: B * C * mst_gated_tiles(T) floats for the backward (nullable when that is 0). States are
+ * float whatever the type. */
+int32_t mst_gated_tiles(int32_t T);
+int mst_gated_fwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,
+                  int64_t gc, const float* h0, const int32_t* lengths, int32_t B, int32_t C, int32_t T,
+                  int32_t reverse, void* h, float* last, float* carry, void* stream);
+/* Gradients of x, gate (contiguous (B, C, T), zero past the lengths) and h0 (nullable), given those
+ * of h (gh: contiguous (B, C, T), nullable) and of last (glast: (B, C), nullable). */
+int mst_gated_bwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,
+                  int64_t gc, const float* h0, const int32_t* lengths, const float* carry,
+                  const void* gh, const float* glast, int32_t B, int32_t C, int32_t T, int32_t reverse,
+                  void* dx, void* dgate, float* dh0, void* stream);
+/* One frame: state (B, C) is updated in place and h (B, C) contiguous receives it; x, gate (B, C)
+ * by batch stride, unit channel stride. */
+int mst_gated_step(int32_t type, const void* x, int64_t xb, const void* gate, int64_t gb, int32_t B,
+                   int32_t C, float* state, void* h, void* stream);
 
 /* ---- elementwise helpers ---- */
 int mst_scale_f32(float* x, int64_t n, float s, void* stream);

@@ -3,6 +3,7 @@
 The product path has no CPU fallback: importing a kernel wrapper without the
 built library, or calling one on a non-CUDA tensor, raises immediately.
 """
+import contextlib
 import ctypes
 import os
 
@@ -19,6 +20,8 @@ MST_OK = 0
 MST_EINVAL = -1000
 ACT_NONE, ACT_RELU, ACT_LRELU = 0, 1, 2
 PAD_REFLECT, PAD_CONSTANT = 0, 1
+# element types of the entry points that take one (MST_F32, MST_BF16, MST_F16)
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class MstSrc(ctypes.Structure):
@@ -80,6 +83,22 @@ SIGNATURES = {
                                   c_float, c_float, c_float, c_float, c_float, c_int32, c_void_p]),
     "mst_adam_dev_f32": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                    c_float, c_float, c_float, c_float, c_void_p]),
+    "mst_grad_norm_workspace_size": (c_size_t, [c_int32]),
+    "mst_grad_norm": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_size_t,
+                                c_void_p]),
+    "mst_grad_scale": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_float, c_void_p]),
+    "mst_adam_clip_f32": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
+                                    c_void_p, c_float, c_float, c_float, c_float, c_float, c_float,
+                                    c_float, c_void_p, c_void_p]),
+    "mst_gated_tiles": (c_int32, [c_int32]),
+    "mst_gated_fwd": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                                c_void_p, c_void_p, c_void_p]),
+    "mst_gated_bwd": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+                                c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mst_gated_step": (c_int32, [c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32,
+                                 c_void_p, c_void_p, c_void_p]),
     "mst_scale_f32": (c_int32, [c_void_p, c_int64, c_float, c_void_p]),
     "mst_fill_f32": (c_int32, [c_void_p, c_int64, c_float, c_void_p]),
     "mst_stft_logpow_f32": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
@@ -142,6 +161,14 @@ def check(rc, what=""):
 
 def stream():
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_SAME = contextlib.nullcontext()
+
+
+def device_of(dev):
+    """Context in which `dev` is the current device (its current stream is then the launch stream)."""
+    return _SAME if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def ptr(t):

@@ -575,3 +575,23 @@ def l1_loss(pred, target):
 def mse_loss(pred, target):
     """nn.MSELoss() forward (test(), train.py:158); evaluation only (torch.ops.mst.mse_loss)."""
     return torch.ops.mst.mse_loss(pred, target)
+
+
+def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
+    """Gated linear recurrence along time, a layer over NCL tensors (torch.ops.mst.gated_recurrence):
+    a_t = sigmoid(gate_t), h_t = a_t h_{t-1} + (1 - a_t) x_t for x, gate (B, C, T), both float32,
+    bfloat16 or float16 and views with unit time stride (the halves of one layer's output) read in
+    place. h0 (B, C): the state before the first frame (None: zeros); with reverse=True time runs
+    from the last frame to the first. lengths (B,): frames at or past a clip's length are not read,
+    give h = 0 and no gradient, and leave the state as it is.
+
+    Returns (h, last): h (B, C, T) in x's type, last (B, C) float32, the state that the next chunk
+    starts from. Differentiable in x, gate and h0; states are float32 inside."""
+    h, last, _ = torch.ops.mst.gated_recurrence(x, gate, h0, lengths, bool(reverse))
+    return h, last
+
+
+def gated_recurrence_step(x, gate, state):
+    """One frame of gated_recurrence for serving: x, gate (B, C); state (B, C) float32 contiguous is
+    updated in place and its new values are returned in x's type. Not differentiable."""
+    return torch.ops.mst.gated_recurrence_step(x, gate, state)

@@ -63,7 +63,8 @@ class GraphedTrainStep:
     """One Adam training step of a flat-buffer PerformanceNet on (x_midi, x_audio, cond,
     target), captured after `warmup` eager steps of the same program. Every call is one real
     training step (the warmup calls included). Requires train.Adam with one parameter group
-    over the model's flat parameters, no overlapped-backward or data-parallel hooks."""
+    over the model's flat parameters, no overlapped-backward or data-parallel hooks. An optimizer
+    with a max_norm clips in the graph too; its grad_norm is then overwritten by every call."""
 
     def __init__(self, model, optimizer, warmup=2):
         if not torch.cuda.is_available():
@@ -97,6 +98,8 @@ class GraphedTrainStep:
         self._lr = float(g["lr"])
         self.hyper = torch.zeros(2, device=dev, dtype=torch.float32)
         self.loss = torch.zeros((), device=dev, dtype=torch.float32)
+        self.max_norm = optimizer.max_norm
+        self.norm = torch.zeros((), device=dev, dtype=torch.float32)
 
     def _state(self):
         st = self.opt._flat_state(0, self.pf, self.params)
@@ -127,7 +130,14 @@ class GraphedTrainStep:
         y = m(*self.inputs[:3])
         loss = torch.ops.mst.l1_loss(y, self.inputs[3])
         loss.backward()
-        K.adam_dev(self.pf, self.gf, st["m"], st["v"], self.hyper, self.b1, self.b2, self.eps)
+        if self.max_norm is None:
+            K.adam_dev(self.pf, self.gf, st["m"], st["v"], self.hyper, self.b1, self.b2, self.eps)
+        else:
+            runs = m.flat_runs()
+            K.grad_norm([self.gf[o:o + n] for o, n in runs], out=self.norm)
+            K.adam_clip(*([x[o:o + n] for o, n in runs] for x in (self.pf, self.gf, st["m"], st["v"])),
+                        self.norm, self.max_norm, 0.0, self.b1, self.b2, self.eps, 1.0, self.hyper)
+            self.opt.grad_norm = self.norm
         self.loss.copy_(loss)
 
     def __call__(self, x_midi, x_audio, cond, target):
@@ -142,6 +152,8 @@ class GraphedTrainStep:
         if lr != self._lr:
             self.lr_dev.fill_(lr)
             self._lr = lr
+        if self.opt.max_norm != self.max_norm:  # a constant of the captured update
+            self.max_norm, self.graph = self.opt.max_norm, None
         st = self._state()
         self.model.train()
         if self.graph is not None:

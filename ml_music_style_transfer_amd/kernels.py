@@ -383,6 +383,216 @@ def adam_dev(p, g, m, v, hyper, b1, b2, eps):
                                     b2, 1.0 - b1, 1.0 - b2, eps, L.stream()), "adam_dev")
 
 
+# ------------------------------------------- gradient norm, clipping, clipped Adam
+def memory_order(t):
+    """Dimension permutation that lists t's dims from the largest stride to the smallest: for a
+    dense tensor, t.permute(perm) is contiguous (a tap-major slot view (d0, d1, k) of (d0, k, d1)
+    memory gives perm (0, 2, 1))."""
+    return sorted(range(t.dim()), key=lambda d: (-t.stride(d), d))
+
+
+def _is_dense(t):
+    return t.is_contiguous() or t.permute(memory_order(t)).is_contiguous()
+
+
+def _grad_table(ts):
+    """(addresses, sizes, element types, count) of dense gradients, as host arrays."""
+    n = len(ts)
+    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]),
+            (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
+            (ctypes.c_int32 * n)(*[L.TYPES[t.dtype] for t in ts]), n)
+
+
+def _check_grads(ts, what):
+    dev = ts[0].device
+    for t in ts:
+        if t.layout != torch.strided or t.dtype not in L.TYPES:
+            raise TypeError(f"{what}: dense float32, bfloat16 or float16 gradients, got {t.dtype} "
+                            f"({t.layout})")
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: CUDA (HIP) tensors only; there is no CPU path")
+        if t.device != dev:
+            raise ValueError(f"{what}: gradients on one device, got {dev} and {t.device}")
+
+
+def check_max_norm(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
+    return max_norm
+
+
+def grad_norm(ts, out=None):
+    """L2 norm over every element of the tensors (0-d float32 on their device; sums in double, in
+    an order that depends on the sizes alone), written to `out` if given."""
+    _check_grads(ts, "grad_norm")
+    dev = ts[0].device
+    with L.device_of(dev):
+        table = _grad_table([t if _is_dense(t) else t.contiguous() for t in ts])
+        norm = torch.empty((), device=dev, dtype=torch.float32) if out is None else out
+        lib = _lib()
+        ws, nb = workspace(lib.mst_grad_norm_workspace_size(table[3]), dev)
+        L.check(lib.mst_grad_norm(*table, L.ptr(norm), L.ptr(ws), nb, L.stream()), "grad_norm")
+    return norm
+
+
+def grad_scale_(ts, norm, max_norm):
+    """g *= min(1, max_norm / (norm + 1e-6)) for every tensor, in place; norm stays on the device."""
+    _check_grads(ts, "clip_grad_norm_")
+    for t in ts:
+        if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise ValueError("clip_grad_norm_: an expanded gradient holds several elements in one "
+                             "place; clone it first")
+    with L.device_of(ts[0].device):
+        dense = [t if _is_dense(t) else t.contiguous() for t in ts]
+        L.check(_lib().mst_grad_scale(*_grad_table(dense), L.ptr(norm), max_norm, L.stream()),
+                "clip_grad_norm_ (gradients that share memory?)")
+        for t, d in zip(ts, dense):
+            if d is not t:
+                t.copy_(d)
+
+
+def adam_clip(ps, gs, ms, vs, norm, max_norm, lr_step, b1, b2, eps, bc2_sqrt, hyper=None):
+    """adam() over lists of float32 tensors, gradients taken times min(1, max_norm / (norm + 1e-6));
+    hyper as in adam_dev(). The four tensors of an entry are dense, in one element order."""
+    n = len(ps)
+    if not len(gs) == len(ms) == len(vs) == n:
+        raise ValueError("adam_clip: as many gradients and moments as parameters")
+    for quad in zip(ps, gs, ms, vs):
+        for t in quad:
+            if t.dtype != torch.float32 or not t.is_cuda:
+                raise TypeError(f"adam_clip: float32 CUDA tensors, got {t.dtype} on {t.device}")
+            if t.numel() != quad[0].numel() or t.device != ps[0].device:
+                raise ValueError("adam_clip: sizes or devices differ")
+    if n == 0:
+        return
+    with L.device_of(ps[0].device):
+        arrays = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in (ps, gs, ms, vs)]
+        numel = (ctypes.c_int64 * n)(*[t.numel() for t in ps])
+        L.check(_lib().mst_adam_clip_f32(*arrays, numel, n, L.ptr(norm), max_norm, lr_step, b2,
+                                         1.0 - b1, 1.0 - b2, eps, bc2_sqrt, L.ptr(hyper), L.stream()),
+                "adam_clip (parameters or moments that share memory?)")
+
+
+# ---------------------------------------------------------- gated linear recurrence
+GATED_TILE = 256  # frames between two kept states (gated.hip; mst_gated_tiles)
+
+
+def gated_tiles(T):
+    return (T + GATED_TILE - 1) // GATED_TILE if T > GATED_TILE else 0
+
+
+def gated_check(x, gate, h0, lengths):
+    """Shapes and types of the recurrence's arguments (real and fake tensors alike)."""
+    if x.dim() != 3 or gate.shape != x.shape:
+        raise ValueError(f"gated_recurrence: x and gate of one shape (B, C, T), got {tuple(x.shape)} "
+                         f"and {tuple(gate.shape)}")
+    if x.dtype not in L.TYPES or gate.dtype != x.dtype:
+        raise TypeError("gated_recurrence: x and gate both float32, bfloat16 or float16, got "
+                        f"{x.dtype} and {gate.dtype}")
+    B, C, T = x.shape
+    if h0 is not None:
+        if tuple(h0.shape) != (B, C):
+            raise ValueError(f"gated_recurrence: h0 must be ({B}, {C}), got {tuple(h0.shape)}")
+        if h0.dtype not in L.TYPES:
+            raise TypeError(f"gated_recurrence: floating h0, got {h0.dtype}")
+    if lengths is not None:
+        if tuple(lengths.shape) != (B,):
+            raise ValueError(f"gated_recurrence: lengths must be ({B},), got {tuple(lengths.shape)}")
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"gated_recurrence: int32 or int64 lengths, got {lengths.dtype}")
+    for t in (gate, h0, lengths):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"gated_recurrence: tensors on one device, got {x.device} and {t.device}")
+
+
+def _unit_time(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _gated_inputs(x, gate, h0, lengths):
+    if not x.is_cuda:
+        raise RuntimeError("gated_recurrence: CUDA (HIP) tensors only; there is no CPU path")
+    if lengths is not None:
+        if lengths.dtype == torch.int64:
+            lengths = lengths.clamp(0, x.shape[2]).to(torch.int32)
+        lengths = lengths.contiguous()
+    return _unit_time(x), _unit_time(gate), h0.float().contiguous() if h0 is not None else None, lengths
+
+
+def _p(t):
+    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def gated_fwd(x, gate, h0, lengths, reverse):
+    """(h, last, carry) of mst_gated_fwd; carry (B, C, gated_tiles(T)) goes to gated_bwd."""
+    gated_check(x, gate, h0, lengths)
+    x, gate, h0, lengths = _gated_inputs(x, gate, h0, lengths)
+    B, C, T = x.shape
+    dev = x.device
+    h = torch.empty(B, C, T, device=dev, dtype=x.dtype)
+    carry = torch.empty(B, C, gated_tiles(T), device=dev, dtype=torch.float32)
+    if h.numel() == 0:  # no frame: the state stays
+        return h, h0.clone() if h0 is not None else torch.zeros(B, C, device=dev), carry
+    last = torch.empty(B, C, device=dev, dtype=torch.float32)
+    with L.device_of(dev):
+        L.check(_lib().mst_gated_fwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
+                                     gate.stride(0), gate.stride(1), _p(h0), _p(lengths), B, C, T,
+                                     1 if reverse else 0, _p(h), _p(last), _p(carry), L.stream()),
+                "gated_recurrence")
+    return h, last, carry
+
+
+def gated_bwd(gh, glast, x, gate, h0, lengths, carry, reverse):
+    """(dx, dgate, dh0) of mst_gated_bwd; gh and glast may be None (zeros)."""
+    gated_check(x, gate, h0, lengths)
+    x, gate, h0, lengths = _gated_inputs(x, gate, h0, lengths)
+    B, C, T = x.shape
+    dev = x.device
+    dx = torch.empty(B, C, T, device=dev, dtype=x.dtype)
+    dgate = torch.empty(B, C, T, device=dev, dtype=x.dtype)
+    gh = gh.to(x.dtype).contiguous() if gh is not None else None
+    glast = glast.float().contiguous() if glast is not None else None
+    if dx.numel() == 0:
+        return dx, dgate, glast.clone() if glast is not None else torch.zeros(B, C, device=dev)
+    dh0 = torch.empty(B, C, device=dev, dtype=torch.float32)
+    with L.device_of(dev):
+        L.check(_lib().mst_gated_bwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
+                                     gate.stride(0), gate.stride(1), _p(h0), _p(lengths), _p(carry),
+                                     _p(gh), _p(glast), B, C, T, 1 if reverse else 0, _p(dx),
+                                     _p(dgate), _p(dh0), L.stream()), "gated_recurrence_backward")
+    return dx, dgate, dh0
+
+
+def gated_step_check(x, gate, state):
+    if x.dim() != 2 or gate.shape != x.shape or state.shape != x.shape:
+        raise ValueError("gated_recurrence_step: x, gate and state of one shape (B, C), got "
+                         f"{tuple(x.shape)}, {tuple(gate.shape)} and {tuple(state.shape)}")
+    if x.dtype not in L.TYPES or gate.dtype != x.dtype:
+        raise TypeError("gated_recurrence_step: x and gate both float32, bfloat16 or float16, got "
+                        f"{x.dtype} and {gate.dtype}")
+    if state.dtype != torch.float32 or not state.is_contiguous():
+        raise TypeError("gated_recurrence_step: a contiguous float32 state (it is updated in place)")
+    if gate.device != x.device or state.device != x.device:
+        raise ValueError("gated_recurrence_step: tensors on one device")
+
+
+def gated_step(x, gate, state):
+    """One frame: state (B, C) updated in place, its new values returned in x's type."""
+    gated_step_check(x, gate, state)
+    if not x.is_cuda:
+        raise RuntimeError("gated_recurrence_step: CUDA (HIP) tensors only; there is no CPU path")
+    x, gate = _unit_time(x), _unit_time(gate)
+    B, C = x.shape
+    h = torch.empty(B, C, device=x.device, dtype=x.dtype)
+    if h.numel():
+        with L.device_of(x.device):
+            L.check(_lib().mst_gated_step(L.TYPES[x.dtype], _p(x), x.stride(0), _p(gate),
+                                          gate.stride(0), B, C, _p(state), _p(h), L.stream()),
+                    "gated_recurrence_step")
+    return h
+
+
 def scale_(x, s):
     L.check(_lib().mst_scale_f32(L.ptr(x), x.numel(), s, L.stream()), "scale")
 

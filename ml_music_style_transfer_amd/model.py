@@ -413,6 +413,19 @@ class PerformanceNet(nn.Module):
         f = self._flat
         return f["param"], f["grad"], f["numel"]
 
+    def flat_runs(self):
+        """[(offset, length)] of the flat buffers without the padding between slots."""
+        f = self._flat
+        if "runs" not in f:
+            runs = []
+            for o, n in sorted(f["index"].values()):
+                if runs and sum(runs[-1]) == o:
+                    runs[-1] = (runs[-1][0], runs[-1][1] + n)
+                else:
+                    runs.append((o, n))
+            f["runs"] = runs
+        return f["runs"]
+
     def _grad_sink(self, on_ready=None):
         f = self._flat
 

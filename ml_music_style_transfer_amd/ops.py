@@ -19,6 +19,8 @@ Python drop-ins use (include/mst.h); there is no CPU implementation (a CPU tenso
   conv1d_k3 (differentiable)         model/model.py:14-22 (nn.Conv1d(k=3, padding=1))
   conv_transpose1d (differentiable)  model/model.py:24-31,242 (nn.ConvTranspose1d, s=2 p=1 / s=1 p=1)
   linear_ncl (differentiable)        model/model.py:98-99,104-107 (nn.Linear over NCL channels)
+  gated_recurrence (differentiable)  none: a layer with a state along time, beside the NCL layers
+  gated_recurrence_step              none: its single frame (the state updated in place)
 
 pad_mode ints: 0 reflect, 1 constant (MST_PAD_*).
 """
@@ -509,8 +511,69 @@ def _linear_backward(ctx, g):
 
 linear_ncl.register_autograd(_linear_backward, setup_context=_conv_setup)
 
+@custom_op("mst::gated_recurrence", mutates_args=())
+def gated_recurrence(x: Tensor, gate: Tensor, h0: Optional[Tensor], lengths: Optional[Tensor],
+                     reverse: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """a_t = sigmoid(gate_t), h_t = a_t h_{t-1} + (1 - a_t) x_t over (B, C, T) from h0 (B, C);
+    frames at or past lengths[b] leave the state and give 0; reverse: t runs down. Returns h in
+    x's type, the final state and the kept states of the backward (B, C, tiles), both float32."""
+    return K.gated_fwd(x, gate, h0, lengths, reverse)
+
+
+@gated_recurrence.register_fake
+def _gated_fake(x, gate, h0, lengths, reverse):
+    K.gated_check(x, gate, h0, lengths)
+    B, C, T = x.shape
+    return (x.new_empty(B, C, T), x.new_empty(B, C, dtype=torch.float32),
+            x.new_empty(B, C, K.gated_tiles(T), dtype=torch.float32))
+
+
+@custom_op("mst::gated_recurrence_backward", mutates_args=())
+def gated_recurrence_backward(grad_h: Optional[Tensor], grad_last: Optional[Tensor], x: Tensor,
+                              gate: Tensor, h0: Optional[Tensor], lengths: Optional[Tensor],
+                              carry: Tensor, reverse: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(d x, d gate, d h0 in float32) of gated_recurrence."""
+    return K.gated_bwd(grad_h, grad_last, x, gate, h0, lengths, carry, reverse)
+
+
+@gated_recurrence_backward.register_fake
+def _gated_bwd_fake(grad_h, grad_last, x, gate, h0, lengths, carry, reverse):
+    B, C, T = x.shape
+    return x.new_empty(B, C, T), x.new_empty(B, C, T), x.new_empty(B, C, dtype=torch.float32)
+
+
+def _gated_setup(ctx, inputs, output):
+    x, gate, h0, lengths, reverse = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, gate, h0, lengths, output[2])
+    ctx.reverse = reverse
+
+
+def _gated_backward(ctx, g_h, g_last, g_carry):
+    x, gate, h0, lengths, carry = ctx.saved_tensors
+    dx, dgate, dh0 = torch.ops.mst.gated_recurrence_backward(g_h, g_last, x, gate, h0, lengths, carry,
+                                                             ctx.reverse)
+    return dx, dgate, dh0.to(h0.dtype) if h0 is not None else None, None, None
+
+
+gated_recurrence.register_autograd(_gated_backward, setup_context=_gated_setup)
+
+
+@custom_op("mst::gated_recurrence_step", mutates_args=("state",))
+def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
+    """One frame of gated_recurrence: x, gate (B, C); state (B, C) float32, updated in place."""
+    return K.gated_step(x, gate, state)
+
+
+@gated_recurrence_step.register_fake
+def _gated_step_fake(x, gate, state):
+    K.gated_step_check(x, gate, state)
+    return x.new_empty(x.shape)
+
+
 OPS = ("stft_logpow", "stft_power", "stft_complex", "istft", "istft_backward", "render_logpow",
        "render_logpow_backward", "melspectrogram",
        "griffinlim", "mss_loss", "l1_loss", "l1_loss_backward", "mse_loss", "onoff", "conv1d_k3",
        "conv1d_k3_backward", "conv_transpose1d", "conv_transpose1d_backward", "linear_ncl",
-       "linear_ncl_backward")
+       "linear_ncl_backward", "gated_recurrence", "gated_recurrence_backward",
+       "gated_recurrence_step")

@@ -48,14 +48,21 @@ class Adam(torch.optim.Optimizer):
     When every parameter of a group with a gradient lives in one PerformanceNet flat
     buffer (and its gradient in the matching flat gradient buffer) the update is one
     kernel launch over the whole buffer; otherwise one launch per parameter.
+
+    max_norm: every step takes the gradients times min(1, max_norm / (norm + 1e-6)), norm being
+    the L2 norm over all gradients of all groups (clip_grad_norm_'s factor). The factor is applied
+    inside the update: p.grad stays as backward left it, and `grad_norm` is the step's norm (a
+    0-d device tensor; reading it waits for the device).
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0,
-                 amsgrad=False):
+                 amsgrad=False, max_norm=None):
         if weight_decay != 0 or amsgrad:
             raise NotImplementedError("the reference uses Adam(lr=1e-3) only (train.py:188)")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=0, amsgrad=False))
         self._flat_groups = {}
+        self.max_norm = None if max_norm is None else K.check_max_norm(max_norm)
+        self.grad_norm = None  # of the last step with a max_norm
 
     def _flat_of(self, group, params):
         """Return (flat_param, flat_grad, numel, offsets) if params tile one model's flat buffers."""
@@ -87,7 +94,11 @@ class Adam(torch.optim.Optimizer):
         """Run this optimizer's update inside the model's backward pass, bucket by bucket
         (BackwardAdam). Only for loops that call step() after every backward (the reference's
         train loop, train.py:131-141): no gradient accumulation across backward passes, no
-        gradient inspection or clipping between backward and step."""
+        gradient inspection or clipping between backward and step (a max_norm needs the norm of
+        all gradients before the first update: refused here)."""
+        if self.max_norm is not None:
+            raise ValueError("Adam.overlap_backward: max_norm clips by the norm of all gradients, "
+                             "known only after backward")
         if model is not None:
             self._owner = model
         self._bwd = BackwardAdam(self, self._owner, bucket_bytes)
@@ -162,6 +173,9 @@ class Adam(torch.optim.Optimizer):
         if bwd is not None and bwd.finish():  # the update already ran inside backward
             self._count_step(bwd.st, bwd.params)
             return loss
+        if self.max_norm is not None:
+            self._clipped_step()
+            return loss
         for gi, group in enumerate(self.param_groups):
             b1, b2 = group["betas"]
             lr, eps = group["lr"], group["eps"]
@@ -191,12 +205,109 @@ class Adam(torch.optim.Optimizer):
                 _adam_param(p, state, lr / bc1, b1, b2, eps, math.sqrt(bc2))
         return loss
 
+    def _clipped_step(self):
+        """step() with a max_norm: the norm over every group's gradients, then each group's update
+        (flat buffers: their ranges between the paddings; otherwise lists of tensors, one launch
+        sequence for the parameters of one step count)."""
+        groups, grads = [], []
+        for gi, group in enumerate(self.param_groups):
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            flat = self._flat_of(group, params)
+            st = self._flat_state(gi, flat[0], params) if flat is not None else None
+            if st is not None:
+                grads += [flat[1][o:o + n] for o, n in self._owner.flat_runs()]
+            else:
+                grads += [p.grad for p in params]
+            if any(t.dtype != torch.float32 for p in params for t in (p, p.grad)):
+                raise TypeError("Adam: float32 parameters and gradients")
+            groups.append((group, params, flat, st))
+        if not groups:
+            return
+        self.grad_norm = K.grad_norm(grads)
+        for group, params, flat, st in groups:
+            b1, b2 = group["betas"]
+            lr, eps = group["lr"], group["eps"]
 
-def _memory_order(t):
-    """Dimension permutation that lists t's dims from the largest stride to the smallest: for a
-    dense tensor, t.permute(perm) is contiguous (a tap-major slot view (d0, d1, k) of (d0, k, d1)
-    memory gives perm (0, 2, 1))."""
-    return sorted(range(t.dim()), key=lambda d: (-t.stride(d), d))
+            def update(tensors, t):
+                K.adam_clip(*zip(*tensors), self.grad_norm, self.max_norm, lr / (1 - b1 ** t), b1, b2,
+                            eps, math.sqrt(1 - b2 ** t))
+
+            if st is not None:
+                pf, gf, _ = flat
+                update([[x[o:o + n] for x in (pf, gf, st["m"], st["v"])] for o, n in
+                        self._owner.flat_runs()], st["step"] + 1)
+                self._count_step(st, params)
+                continue
+            by_step, copied = {}, []
+            for p in params:
+                state = self.state[p]
+                if len(state) == 0 or state.get("exp_avg") is None:
+                    state["step"] = torch.tensor(0.0)
+                    state["exp_avg"] = torch.zeros_like(p)
+                    state["exp_avg_sq"] = torch.zeros_like(p)
+                state["step"] += 1
+                pv, g, mv, vv, back = _adam_views(p, state)
+                by_step.setdefault(float(state["step"]), []).append((pv, g, mv, vv))
+                copied += back
+            for t, tensors in by_step.items():
+                update(tensors, t)
+            for dst, src in copied:
+                dst.copy_(src)
+
+
+_memory_order = K.memory_order
+
+
+def _grads_of(parameters, what):
+    """(parameters, gradients) of those that have one; data-parallel averages have landed."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    params = [p for p in parameters if p.grad is not None]
+    if len({id(p) for p in params}) != len(params):
+        raise ValueError(f"{what}: a parameter is listed twice")
+    for owner in {id(o): o for o in (_owner(p) for p in params) if o is not None}.values():
+        dp.finish_gradients(owner)
+    return params, [p.grad for p in params]
+
+
+def _owner(p):
+    ref = getattr(p, "_mst_flat_owner", None)
+    return ref() if ref is not None else None
+
+
+@torch.no_grad()
+def grad_norm(parameters):
+    """L2 norm over the gradients of all parameters as one vector (0-d float32 device tensor; no
+    host synchronisation). Parameters without a gradient are left out; gradients may be float32,
+    bfloat16 and float16, mixed, of any strides, on one device."""
+    _, grads = _grads_of(parameters, "grad_norm")
+    return K.grad_norm(grads) if grads else torch.tensor(0.0)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ on the device: every gradient times
+    min(1, max_norm / (norm + 1e-6)), in place; returns the norm before (as grad_norm). Only the L2
+    norm is offered. error_if_nonfinite=True waits for the norm and raises before a gradient is
+    changed. Adam(max_norm=...) clips inside the update instead, without this pass."""
+    if float(norm_type) != 2.0:
+        raise ValueError(f"clip_grad_norm_: the L2 norm only (norm_type=2.0), got {norm_type}")
+    max_norm = K.check_max_norm(max_norm)
+    params, grads = _grads_of(parameters, "clip_grad_norm_")
+    if not grads:
+        return torch.tensor(0.0)
+    for p in params:
+        hook = getattr(_owner(p), "_mst_adam", None)
+        if hook is not None and hook.active and hook.launched:
+            raise RuntimeError("clip_grad_norm_: the update of these gradients ran inside backward "
+                               "(Adam.overlap_backward)")
+    norm = K.grad_norm(grads)
+    if error_if_nonfinite and not math.isfinite(norm.item()):
+        raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {norm.item()}")
+    K.grad_scale_(grads, norm, max_norm)
+    return norm
 
 
 def _adam_param(p, state, lr_step, b1, b2, eps, bc2_sqrt):
@@ -204,6 +315,15 @@ def _adam_param(p, state, lr_step, b1, b2, eps, bc2_sqrt):
     moments are handed over in p's memory order: the gradient (any layout) is permuted into it,
     the moments are re-laid-out to p's strides once if they differ (e.g. loaded from a
     checkpoint), and a non-dense p is updated through a contiguous copy."""
+    pv, g, mv, vv, back = _adam_views(p, state)
+    K.adam(pv, g, mv, vv, lr_step, b1, b2, eps, bc2_sqrt)
+    for dst, src in back:
+        dst.copy_(src)
+
+
+def _adam_views(p, state):
+    """(p, gradient, moments) of one parameter as dense tensors in p's memory order, and the
+    [(destination, copy)] to write back after an update that ran on copies."""
     for key in ("exp_avg", "exp_avg_sq"):
         x = state[key]
         if x.stride() != p.stride():
@@ -215,13 +335,9 @@ def _adam_param(p, state, lr_step, b1, b2, eps, bc2_sqrt):
     mv, vv = state["exp_avg"].permute(perm), state["exp_avg_sq"].permute(perm)
     g = p.grad.permute(perm).contiguous()
     if pv.is_contiguous() and mv.is_contiguous() and vv.is_contiguous():
-        K.adam(pv, g, mv, vv, lr_step, b1, b2, eps, bc2_sqrt)
-        return
+        return pv, g, mv, vv, []
     pc, mc, vc = pv.contiguous(), mv.contiguous(), vv.contiguous()
-    K.adam(pc, g, mc, vc, lr_step, b1, b2, eps, bc2_sqrt)
-    pv.copy_(pc)
-    mv.copy_(mc)
-    vv.copy_(vc)
+    return pc, g, mc, vc, [(pv, pc), (mv, mc), (vv, vc)]
 
 
 class BackwardAdam:
@@ -261,7 +377,7 @@ class BackwardAdam:
 
     def _eligible(self):
         m = self.model
-        if len(self.opt.param_groups) != 1 or not m._flat_ok():
+        if len(self.opt.param_groups) != 1 or not m._flat_ok() or self.opt.max_norm is not None:
             return False
         # the group may also hold parameters outside the flat buffer (the dead MBR convolutions,
         # model.py:143-174): backward never gives them a gradient, so Adam skips them anyway
@@ -339,10 +455,11 @@ class BackwardAdam:
         return True
 
 
-def make_optimizer(model, lr=1e-3, overlap_backward=False):
+def make_optimizer(model, lr=1e-3, overlap_backward=False, max_norm=None):
     """optim.Adam(model.parameters(), lr=1e-3) (train.py:188) bound to the model's flat buffers;
-    overlap_backward=True runs its update inside backward (BackwardAdam)."""
-    opt = Adam(model.parameters(), lr=lr).attach(model)
+    overlap_backward=True runs its update inside backward (BackwardAdam); max_norm clips the
+    gradients inside the update (Adam)."""
+    opt = Adam(model.parameters(), lr=lr, max_norm=max_norm).attach(model)
     return opt.overlap_backward() if overlap_backward else opt
 
 
@@ -497,7 +614,9 @@ def main(args, return_model=False):
         model._seed += rank << 24              # per-rank dropout streams
     # the reference loop steps after every backward (train.py:131-141), so the update runs per
     # bucket inside backward (BackwardAdam: bitwise the one-launch update, 1.5-2.3 % faster)
-    optimizer = make_optimizer(model, lr=1e-3, overlap_backward=True)
+    # (a clip needs the norm of all gradients first: the update then follows backward)
+    clip = getattr(args, "clip_norm", None)
+    optimizer = make_optimizer(model, lr=1e-3, overlap_backward=clip is None, max_norm=clip)
     model.zero_grad()
     optimizer.zero_grad()
     scheduler = torch.optim.lr_scheduler.ReduceLROnPlateau(optimizer, 'min')
@@ -566,6 +685,8 @@ def parse_args(argv=None):
                         help="phase that renders the prediction for the multi-scale loss")
     parser.add_argument("-gl-iters", type=int, default=8,
                         help="Griffin-Lim iterations behind the multi-scale loss's audio")
+    parser.add_argument("-clip-norm", type=float, default=None,
+                        help="limit of the gradients' global L2 norm (default: no clipping)")
     return parser.parse_args(argv)
 
 
@@ -573,5 +694,5 @@ if __name__ == "__main__":
     main(parse_args())
 
 
-__all__ = ["train", "test", "Adam", "make_optimizer", "make_loss", "LOSSES", "hyperparams", "main",
+__all__ = ["train", "test", "Adam", "make_optimizer", "grad_norm", "clip_grad_norm_", "make_loss", "LOSSES", "hyperparams", "main",
            "np"]

@@ -8,6 +8,8 @@ CPU restatements of the reference's hot path (silburt/ML_Music_Style_Transfer):
                    tests/test_griffinlim.py:23, tests/plot_spec.py:20)
   midi_ref.py      framing constants, chunk formulas, piano-roll/onoff rules
                    (preprocessing/preprocess.py:17-42, 60-96, 118-160)
+  gated_ref.py     gated linear recurrence and its gradients, float64, with float32 error bounds
+  clip_ref.py      gradient norm, clipping, clipped Adam, float64, with float32 error bounds
 
 Only tests/, __graft_entry__.smoke() and bench.py's cpu_baseline leg may import
 anything here, and only as the checker / CPU baseline. The product package
