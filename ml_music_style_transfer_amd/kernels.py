@@ -475,7 +475,7 @@ def adam_clip(ps, gs, ms, vs, norm, max_norm, lr_step, b1, b2, eps, bc2_sqrt, hy
 
 
 # ---------------------------------------------------------- gated linear recurrence
-GATED_TILE = 256  # frames between two kept states (gated.hip; mst_gated_tiles)
+GATED_TILE = 512  # frames between two kept states (gated.hip; mst_gated_tiles)
 
 
 def gated_tiles(T):

@@ -3,13 +3,13 @@ on what a float32 evaluation of the same formulas, in any order of composition, 
 
   a_t = sigmoid(gate_t), c_t = 1 - a_t, h_t = a_t h_{t-1} + c_t x_t; frames t >= length are the identity
 
-Error model, u = 2^-24 (half a float32 step): exp within 2u, 1 + e, the quotient and e r one rounding
-each give a and c to 6u; c x to 7u. A state of magnitude M (the recurrence run on |x|, |h0|) that passes a
-frame gains at most a's 6u and two roundings, and the frame's own term its 7u and the sum's rounding;
-composing maps in a tree rounds a term at most once a level, and a term has passed at least as many
-frames as levels. So
+Error model, u = 2^-24 (half a float32 step): an exponential within 4u, 1 + e, the quotient and e r one
+rounding each give a and c to 9u; c x to 10u. A state of magnitude M (the recurrence run on |x|, |h0|)
+that passes a frame gains at most a's 9u and two roundings, 11u a M in all; the frame's own term its 10u
+and the sum's rounding; composing maps in a tree rounds a term at most once a level, and a term has
+passed at least as many frames as levels. With M_t = a_t M_{t-1} + c_t |x_t| both are within
   E_t = a_t (E_{t-1} + 8u M_{t-1}) + 12u c_t |x_t| + 4u M_t
-and the same for what is handed back, u_t = a_t (gh_t + u_{t+1}).
+and what is handed back, u_t = a_t (gh_t + u_{t+1}), is of the same form.
 """
 import torch
 

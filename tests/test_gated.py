@@ -69,7 +69,7 @@ def test_fake_shapes_and_tiles():
         x = torch.empty(2, 5, 600, device="cuda", dtype=torch.bfloat16)
         h, last, carry = torch.ops.mst.gated_recurrence(x, x, None, None, False)
         assert h.shape == x.shape and h.dtype == x.dtype
-        assert last.shape == (2, 5) and last.dtype == torch.float32 and carry.shape == (2, 5, 3)
+        assert last.shape == (2, 5) and last.dtype == torch.float32 and carry.shape == (2, 5, K.gated_tiles(600))
         dx, dg, dh0 = torch.ops.mst.gated_recurrence_backward(h, last, x, x, None, None, carry, False)
         assert dx.shape == dg.shape == x.shape and dh0.shape == (2, 5)
         s = torch.empty(2, 5, device="cuda")
