@@ -226,7 +226,7 @@ int mst_adam_clip_f32(float* const* p, const float* const* g, float* const* m, f
 /* ---- gated linear recurrence over time, element type `type` (MST_F32 / MST_BF16 / MST_F16) ----
  *   a_t = sigmoid(gate_t);  h_t = a_t h_{t-1} + (1 - a_t) x_t,  h_{-1} = h0 (nullable: zeros)
  * x, gate: (B, C, T) by batch and channel strides (elements), unit time stride. lengths (nullable,
- * B on the device, taken into [0, T]): frames at or past lengths[b] are not read, leave the state
+ * B on the device, taken into [0, T]): frames at or past lengths[b] are not used, leave the state
  * as it is and give h = 0. reverse != 0: t runs from the last frame down, h0 enters there.
  * h: (B, C, T) contiguous; last (B, C): the state after the last frame (the first when reversed).
  * carry: B * C * mst_gated_tiles(T) floats for the backward (nullable when that is 0). States are

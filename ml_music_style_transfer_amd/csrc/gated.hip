@@ -6,7 +6,7 @@
 // A frame is the affine map h -> a h + b, b = (1 - a) x, and maps compose associatively:
 // (a2, b2) after (a1, b1) = (a2 a1, a2 b1 + b2). A row (b, c) belongs to a group of W lanes, each
 // lane to V = 8 consecutive frames: the lane composes its maps, the group scans the compositions
-// (DPP row shifts: no LDS for 16 lanes, a scan costs about 4 VALU a level), and each lane then runs
+// (DPP row shifts: two instructions a level and no LDS within 16 lanes), and each lane then runs
 // its frames from the state that enters them. W lanes x V frames are a tile; longer rows walk their
 // tiles with the state in a register and the next tile's loads in flight. Everything between the
 // loads and the stores is 32-bit float.
@@ -46,22 +46,52 @@ template <> struct Piece<float> { typedef float t __attribute__((ext_vector_type
 template <> struct Piece<__bf16> { typedef __bf16 t __attribute__((ext_vector_type(8), aligned(2))); };
 template <> struct Piece<_Float16> { typedef _Float16 t __attribute__((ext_vector_type(8), aligned(2))); };
 
-// a lane's V frames as they lie in memory: converted after the next tile's loads are under way
-template <typename T> struct Raw {
+// A lane's V frames as they lie in memory: converted after the next tile's loads are under way.
+// Loads are free of branches (at a join the compiler would wait for their data): a piece that ends
+// past `end` reads the last 16 bytes before it, and settle() moves what belongs to the lane down.
+// Frames past the clip hold anything. `end` is the clip's length, or P in a shorter clip: the row
+// has T >= P frames. SHORT: rows of T < P frames, read frame by frame.
+template <typename T, bool SHORT> struct Raw {
   static constexpr int P = 16 / sizeof(T), N = V / P;
   typename Piece<T>::t q[N];
 
-  // frames [t, t + V) of a row; those from `end` on hold anything (nothing there is read)
   __device__ __forceinline__ void load(const T* row, int t, int end) {
+    if constexpr (SHORT) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int s = t + i * P;
-      if (s + P <= end) {
-        q[i] = *reinterpret_cast<const typename Piece<T>::t*>(row + s);
-      } else if (s < end) {
+      for (int k = 0; k < P; ++k) q[0][k] = row[min(t + k, end - 1)];
 #pragma unroll
-        for (int k = 0; k < P; ++k) q[i][k] = row[min(s + k, end - 1)];
+      for (int i = 1; i < N; ++i) q[i] = q[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        q[i] = *reinterpret_cast<const typename Piece<T>::t*>(row + max(min(t + i * P, end - P), 0));
+    }
+  }
+  __device__ __forceinline__ void settle(int t, int end) {
+    if constexpr (!SHORT) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int n = t + i * P - (end - P);
+        if (0 < n && n < P) down(q[i], n);
       }
+    }
+  }
+  // q[k] <- q[k + n], 0 < n < P, by the bits of n (as words where n allows)
+  static __device__ __forceinline__ void down(typename Piece<T>::t& q, int n) {
+    if constexpr (P == 8) {
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+      u32x4 w = __builtin_bit_cast(u32x4, q);
+      if (n & 4) w[0] = w[2], w[1] = w[3];
+      if (n & 2) w[0] = w[1], w[1] = w[2], w[2] = w[3];
+      if (n & 1) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) w[k] = __builtin_amdgcn_alignbit(w[k + 1], w[k], 16);
+        w[3] >>= 16;
+      }
+      q = __builtin_bit_cast(typename Piece<T>::t, w);
+    } else {
+      if (n & 2) q[0] = q[2], q[1] = q[3];
+      if (n & 1) q[0] = q[1], q[1] = q[2], q[2] = q[3];
     }
   }
   __device__ __forceinline__ float operator[](int k) const { return (float)q[k / P][k % P]; }
@@ -73,33 +103,58 @@ __device__ __forceinline__ void store(T* row, int t, int end, const float (&v)[V
 #pragma unroll
   for (int i = 0; i < V / P; ++i) {
     const int s = t + i * P;
+    if (s >= end) break;
+    typename Piece<T>::t q;
+#pragma unroll
+    for (int k = 0; k < P; ++k) q[k] = (T)v[i * P + k];
     if (s + P <= end) {
-      typename Piece<T>::t q;
-#pragma unroll
-      for (int k = 0; k < P; ++k) q[k] = (T)v[i * P + k];
       *reinterpret_cast<typename Piece<T>::t*>(row + s) = q;
-    } else {
-#pragma unroll
-      for (int k = 0; k < P; ++k)
-        if (s + k < end) row[s + k] = (T)v[i * P + k];
+    } else {  // the row's end, by the bits of what is left
+      int n = end - s;
+      T* to = row + s;
+      if constexpr (P == 8) {
+        if (n & 4) {
+          typedef T half __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+          *reinterpret_cast<half*>(to) = half{q[0], q[1], q[2], q[3]};
+          q[0] = q[4], q[1] = q[5], q[2] = q[6];
+          to += 4;
+        }
+      }
+      if (n & 2) {
+        to[0] = q[0], to[1] = q[1];
+        q[0] = q[2];
+        to += 2;
+      }
+      if (n & 1) to[0] = q[0];
     }
   }
 }
 
 // a = sigmoid(g) and c = 1 - a, each to its own relative precision (c is not formed from a).
-// e^-m = 2^t e^(-m - t ln 2) with t = -m log2(e) rounded: the second factor is 1 + a rounding's
-// size. Past 150 the first is 0, as it is for infinite g; a g that is not a number stays none.
+// e^-|g| = 2^t e^(-|g| - t ln 2) with t = -|g| log2(e) rounded: the second factor is 1 + a rounding's
+// size (taken into [-1, 1], since an infinite g makes its exponent no number where 2^t is zero; of a
+// g that is no number 2^t is none either). The quotient is the hardware's, to its last place.
 __device__ __forceinline__ void gate_of(float g, float& a, float& c) {
-  const float m = fabsf(g) > 150.f ? 150.f : fabsf(g);
-  const float t = m * -1.44269504f;
+  const float t = fabsf(g) * -1.44269504f;
   float e = __builtin_amdgcn_exp2f(t);
-  e = fmaf(e, fmaf(t, -0.693147181f, -m), e);
-  const float d = 1.f + e;
-  float r = __builtin_amdgcn_rcpf(d);
-  r = fmaf(r, fmaf(-d, r, 1.f), r);  // one Newton step: the quotient to half a step
+  e = fmaf(e, __builtin_amdgcn_fmed3f(fmaf(t, -0.693147181f, -fabsf(g)), -1.f, 1.f), e);
+  const float r = __builtin_amdgcn_rcpf(1.f + e);
   const float er = e * r;
   a = g < 0.f ? er : r;
   c = g < 0.f ? r : er;
+}
+
+// frames from `n` on become the identity: an infinite gate holds the state, and x adds nothing
+__device__ __forceinline__ void hold(int n, float (&g)[V], float (&x)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    g[k] = k < n ? g[k] : __builtin_inff();
+    x[k] = k < n ? x[k] : 0.f;
+  }
+}
+__device__ __forceinline__ void clear(int n, float (&v)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = k < n ? v[k] : 0.f;
 }
 
 // lane's value from the lane that the DPP control names, `old` where it names none
@@ -117,14 +172,12 @@ template <int W, bool DOWN, int D>
 __device__ __forceinline__ void level(float& A, float& H) {
   const int lane = threadIdx.x & 63;
   float a, h;
-  if constexpr (D < 16) {
+  if constexpr (D < 16) {  // several groups in a row of 16 lanes
+    const bool in = DOWN ? (lane & (W - 1)) + D < W : (lane & (W - 1)) >= D;
     a = dpp<(DOWN ? kRowShl : kRowShr) + D>(1.f, A);
     h = dpp<(DOWN ? kRowShl : kRowShr) + D>(0.f, H);
-    if constexpr (W < 16) {  // a row of 16 lanes holds several groups
-      const bool in = DOWN ? (lane & (W - 1)) + D < W : (lane & (W - 1)) >= D;
-      a = in ? a : 1.f;
-      h = in ? h : 0.f;
-    }
+    a = in ? a : 1.f;
+    h = in ? h : 0.f;
   } else if constexpr (!DOWN) {  // the last lane of the 16 (32) lanes before, for every second 16 (32)
     a = dpp<D == 16 ? kBcast15 : kBcast31, D == 16 ? 0xa : 0xc>(1.f, A);
     h = dpp<D == 16 ? kBcast15 : kBcast31, D == 16 ? 0xa : 0xc>(0.f, H);
@@ -140,15 +193,37 @@ __device__ __forceinline__ void level(float& A, float& H) {
   A *= a;
 }
 
-// Scan of the lanes' maps (A, H) over the W lanes of a row, in lane order or against it. In: a
-// lane's own map. Out: the composition of the maps before it (the first lane: the identity); for
-// a whole wave also that of the row in (At, Ht).
+// Levels 1 to 8 as fused DPP instructions, for groups of 16 lanes or more: a lane whose source is
+// outside its row of 16 is not written, which is the identity. A DPP operand may be read two
+// instructions after it is written at the earliest: two independent scans keep each other's
+// distance, one alone waits.
+#define MST_FMAC(H, A, C) "v_fmac_f32_dpp " H ", " H ", " A " " C " row_mask:0xf bank_mask:0xf\n\t"
+#define MST_MUL(A, C) "v_mul_f32_dpp " A ", " A ", " A " " C " row_mask:0xf bank_mask:0xf\n\t"
+#define MST_ONE(C) MST_FMAC("%0", "%1", C) MST_MUL("%1", C) "s_nop 1\n\t"
+#define MST_TWO(C, D) MST_FMAC("%0", "%1", C) MST_MUL("%1", C) MST_FMAC("%2", "%3", D) MST_MUL("%3", D)
+template <bool DOWN>
+__device__ __forceinline__ void levels16(float& A, float& H) {
+  if constexpr (DOWN)
+    asm volatile("s_nop 1\n\t" MST_ONE("row_shl:1") MST_ONE("row_shl:2") MST_ONE("row_shl:4") MST_ONE("row_shl:8")
+                 : "+v"(H), "+v"(A));
+  else
+    asm volatile("s_nop 1\n\t" MST_ONE("row_shr:1") MST_ONE("row_shr:2") MST_ONE("row_shr:4") MST_ONE("row_shr:8")
+                 : "+v"(H), "+v"(A));
+}
+// (A, H) in lane order and (B, K) against it
+__device__ __forceinline__ void levels16_two(float& A, float& H, float& B, float& K) {
+  asm volatile("s_nop 1\n\t" MST_TWO("row_shr:1", "row_shl:1") MST_TWO("row_shr:2", "row_shl:2")
+               MST_TWO("row_shr:4", "row_shl:4") MST_TWO("row_shr:8", "row_shl:8") "s_nop 1"
+               : "+v"(H), "+v"(A), "+v"(K), "+v"(B));
+}
+#undef MST_FMAC
+#undef MST_MUL
+#undef MST_ONE
+#undef MST_TWO
+
+// The levels above 8, the row's total and the step from "up to this lane" to "before it".
 template <int W, bool DOWN>
-__device__ __forceinline__ void scan(float& A, float& H, float& At, float& Ht) {
-  level<W, DOWN, 1>(A, H);
-  level<W, DOWN, 2>(A, H);
-  if constexpr (W > 4) level<W, DOWN, 4>(A, H);
-  if constexpr (W > 8) level<W, DOWN, 8>(A, H);
+__device__ __forceinline__ void finish_scan(float& A, float& H, float& At, float& Ht) {
   if constexpr (W > 16) level<W, DOWN, 16>(A, H);
   if constexpr (W > 32) {
     level<W, DOWN, 32>(A, H);
@@ -159,6 +234,36 @@ __device__ __forceinline__ void scan(float& A, float& H, float& At, float& Ht) {
   H = dpp<DOWN ? kWaveShl1 : kWaveShr1>(0.f, H);
   if constexpr (W < 64)
     if ((threadIdx.x & (W - 1)) == (DOWN ? W - 1 : 0)) A = 1.f, H = 0.f;
+}
+
+// Scan of the lanes' maps (A, H) over the W lanes of a row, in lane order or against it. In: a
+// lane's own map. Out: the composition of the maps before it (the first lane: the identity); for
+// a whole wave also that of the row in (At, Ht).
+template <int W, bool DOWN>
+__device__ __forceinline__ void scan(float& A, float& H, float& At, float& Ht) {
+  if constexpr (W >= 16) {
+    levels16<DOWN>(A, H);
+  } else {
+    level<W, DOWN, 1>(A, H);
+    level<W, DOWN, 2>(A, H);
+    if constexpr (W > 4) level<W, DOWN, 4>(A, H);
+  }
+  finish_scan<W, DOWN>(A, H, At, Ht);
+}
+
+// scan of (A, H) with DOWN and of (B, K) against it; (Bt, Kt) is the second's total
+template <int W, bool DOWN>
+__device__ __forceinline__ void scan_two(float& A, float& H, float& B, float& K, float& Bt, float& Kt) {
+  float At, Ht;
+  if constexpr (W >= 16) {
+    if constexpr (DOWN) levels16_two(B, K, A, H);
+    else levels16_two(A, H, B, K);
+    finish_scan<W, DOWN>(A, H, At, Ht);
+    finish_scan<W, !DOWN>(B, K, Bt, Kt);
+  } else {
+    scan<W, DOWN>(A, H, At, Ht);
+    scan<W, !DOWN>(B, K, Bt, Kt);
+  }
 }
 
 // the rows of x and gate, and the clip's length, of row `row`
@@ -181,42 +286,48 @@ __device__ __forceinline__ uint32_t group_id() {
   return W == 64 ? __builtin_amdgcn_readfirstlane(i) : i;
 }
 
-template <typename T, int W, bool REV>
+// W lanes a row; MULTI: more than one tile (W = 64); SHORT: rows shorter than a piece (W = 4)
+template <typename T, int W, bool REV, bool MULTI, bool SHORT>
 __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
   const uint32_t row = group_id<W>();
   if (row >= p.rows) return;
   const int lane = threadIdx.x & (W - 1);
   const Row<T> r(p, row);
+  const int end = SHORT ? p.T : max(r.len, 16 / (int)sizeof(T));
   T* h = (T*)p.h + (long long)row * p.T;
   float s = p.h0 ? p.h0[row] : 0.f;
-  int t = (REV ? p.tiles - 1 : 0) * (W * V) + lane * V;
-  Raw<T> xr, gr;
-  xr.load(r.x, t, r.len);
-  gr.load(r.g, t, r.len);
-  for (int i = 0; i < p.tiles; ++i) {
-    if (W == 64 && p.tiles > 1 && lane == 0)
-      p.carry[(long long)row * p.tiles + (REV ? p.tiles - 1 - i : i)] = s;
-    float b[V], a[V], c[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      b[k] = xr[k];
-      gate_of(gr[k], a[k], c[k]);
-    }
+  int t = (MULTI && REV ? p.tiles - 1 : 0) * kTile + lane * V;
+  struct Tile {
+    Raw<T, SHORT> x, g;
+  } u, v;
+  u.x.load(r.x, t, end);
+  u.g.load(r.g, t, end);
+  int i = 0;
+  // one tile; the next one's loads go to registers of their own (copies would wait for them)
+  auto step = [&](Tile& tile, Tile& next) __attribute__((always_inline)) {
+    if (MULTI && lane == 0) p.carry[(long long)row * p.tiles + (REV ? p.tiles - 1 - i : i)] = s;
+    float b[V], g[V], a[V], c[V];
     const int now = t;
-    if (W == 64 && i + 1 < p.tiles) {
+    if (MULTI) {
       t += REV ? -kTile : kTile;
-      xr.load(r.x, t, r.len);
-      gr.load(r.g, t, r.len);
+      next.x.load(r.x, t, end);
+      next.g.load(r.g, t, end);
+      if (now - lane * V >= r.len) {  // a tile past the clip's end
+        clear(0, b);
+        store(h, now, p.T, b);
+        return;
+      }
     }
-    if (now + V > r.len) {
+    tile.x.settle(now, end);
+    tile.g.settle(now, end);
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (now + k >= r.len) a[k] = 1.f, b[k] = c[k] = 0.f;
-    }
+    for (int k = 0; k < V; ++k) b[k] = tile.x[k], g[k] = tile.g[k];
+    if (now + V > r.len) hold(r.len - now, g, b);
     float A = 1.f, H = 0.f, At, Ht;
 #pragma unroll
     for (int q = 0; q < V; ++q) {
       const int k = REV ? V - 1 - q : q;
+      gate_of(g[k], a[k], c[k]);
       b[k] *= c[k];
       H = fmaf(a[k], H, b[k]);
       A *= a[k];
@@ -231,57 +342,63 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
       b[k] = e;
     }
     if (W < 64) s = e;
-    if (now + V > r.len) {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (now + k >= r.len) b[k] = 0.f;
-    }
+    if (r.len < p.T && now + V > r.len) clear(r.len - now, b);
     store(h, now, p.T, b);
+  };
+  step(u, v);
+  while (MULTI && ++i < p.tiles) {
+    step(v, u);
+    if (++i == p.tiles) break;
+    step(u, v);
   }
   if (lane == (W == 64 || REV ? 0 : W - 1)) p.last[row] = s;
 }
 
-template <typename T, int W, bool REV>
+template <typename T, int W, bool REV, bool MULTI, bool SHORT>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
   const uint32_t row = group_id<W>();
   if (row >= p.rows) return;
   const int lane = threadIdx.x & (W - 1);
   const Row<T> r(p, row);
+  const int end = SHORT ? p.T : max(r.len, 16 / (int)sizeof(T));
   const T* gh = p.gh ? (const T*)p.gh + (long long)row * p.T : r.x;
-  const int ghlen = p.gh ? r.len : 0;
   float s = p.glast ? p.glast[row] : 0.f;
   const float h0 = p.h0 ? p.h0[row] : 0.f;
-  int t = (REV ? 0 : p.tiles - 1) * (W * V) + lane * V;
-  Raw<T> xr, gr, dr;
-  xr.load(r.x, t, r.len);
-  gr.load(r.g, t, r.len);
-  dr.load(gh, t, ghlen);
-  for (int i = 0; i < p.tiles; ++i) {
-    const float in = W == 64 && p.tiles > 1
-                         ? p.carry[(long long)row * p.tiles + (REV ? i : p.tiles - 1 - i)] : h0;
-    float x[V], d[V], a[V], c[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      x[k] = xr[k];
-      d[k] = dr[k];
-      gate_of(gr[k], a[k], c[k]);
-    }
+  int t = (MULTI && !REV ? p.tiles - 1 : 0) * kTile + lane * V;
+  struct Tile {
+    Raw<T, SHORT> x, g, d;
+  } v, w;
+  v.x.load(r.x, t, end);
+  v.g.load(r.g, t, end);
+  v.d.load(gh, t, end);
+  int i = 0;
+  auto step = [&](Tile& tile, Tile& next) __attribute__((always_inline)) {
+    const float in = MULTI ? p.carry[(long long)row * p.tiles + (REV ? i : p.tiles - 1 - i)] : h0;
+    float x[V], g[V], d[V], a[V], c[V];
     const int now = t;
-    if (W == 64 && i + 1 < p.tiles) {
+    if (MULTI) {
       t += REV ? kTile : -kTile;
-      xr.load(r.x, t, r.len);
-      gr.load(r.g, t, r.len);
-      dr.load(gh, t, ghlen);
+      next.x.load(r.x, t, end);
+      next.g.load(r.g, t, end);
+      next.d.load(gh, t, end);
+      if (now - lane * V >= r.len) {  // a tile past the clip's end
+        clear(0, x);
+        store((T*)p.dx + (long long)row * p.T, now, p.T, x);
+        store((T*)p.dgate + (long long)row * p.T, now, p.T, x);
+        return;
+      }
     }
+    tile.x.settle(now, end);
+    tile.g.settle(now, end);
+    tile.d.settle(now, end);
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[k] = tile.x[k], g[k] = tile.g[k], d[k] = p.gh ? tile.d[k] : 0.f;
     if (now + V > r.len) {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (now + k >= r.len) a[k] = 1.f, c[k] = x[k] = d[k] = 0.f;
+      hold(r.len - now, g, x);
+      clear(r.len - now, d);
     }
-    if (!p.gh) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) d[k] = 0.f;
-    }
+    for (int k = 0; k < V; ++k) gate_of(g[k], a[k], c[k]);
     float A = 1.f, H = 0.f, U = 0.f, At, Ht;
 #pragma unroll
     for (int q = 0; q < V; ++q) {
@@ -291,10 +408,9 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
       U = a[j] * (d[j] + U);
     }
     float Ua = A;
-    scan<W, REV>(A, H, At, Ht);
-    scan<W, !REV>(Ua, U, At, Ht);
-    float e = fmaf(A, in, H);   // the state before the lane's first frame
-    float u = fmaf(Ua, s, U);   // what the frame after the lane's last hands back
+    scan_two<W, REV>(A, H, Ua, U, At, Ht);
+    float e = fmaf(A, in, H);  // the state before the lane's first frame
+    float u = fmaf(Ua, s, U);  // what the frame after the lane's last hands back
     if (W == 64) s = fmaf(At, s, Ht);
     float diff[V];
 #pragma unroll
@@ -312,13 +428,18 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
       diff[k] *= u * c[k];
     }
     if (W < 64) s = u;
-    if (now + V > r.len) {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (now + k >= r.len) x[k] = diff[k] = 0.f;
+    if (r.len < p.T && now + V > r.len) {
+      clear(r.len - now, x);
+      clear(r.len - now, diff);
     }
     store((T*)p.dx + (long long)row * p.T, now, p.T, x);
     store((T*)p.dgate + (long long)row * p.T, now, p.T, diff);
+  };
+  step(v, w);
+  while (MULTI && ++i < p.tiles) {
+    step(w, v);
+    if (++i == p.tiles) break;
+    step(v, w);
   }
   if (p.dh0 && lane == (W == 64 || !REV ? 0 : W - 1)) p.dh0[row] = s;
 }
@@ -351,16 +472,18 @@ template <typename T, bool REV, bool BWD>
 void launch_w(const Args& p, hipStream_t st) {
   const int w = lanes_of(p.T);
   const dim3 grid((unsigned)(((long long)p.rows * w + 255) / 256));
-#define MST_GATED(W_)                                                                        \
-  do {                                                                                       \
-    if (BWD) hipLaunchKernelGGL((gated_bwd_kernel<T, W_, REV>), grid, dim3(256), 0, st, p);  \
-    else hipLaunchKernelGGL((gated_fwd_kernel<T, W_, REV>), grid, dim3(256), 0, st, p);      \
+#define MST_GATED(W_, MULTI, SHORT)                                                                        \
+  do {                                                                                                     \
+    if (BWD) hipLaunchKernelGGL((gated_bwd_kernel<T, W_, REV, MULTI, SHORT>), grid, dim3(256), 0, st, p);  \
+    else hipLaunchKernelGGL((gated_fwd_kernel<T, W_, REV, MULTI, SHORT>), grid, dim3(256), 0, st, p);      \
   } while (0)
-  if (w == 4) MST_GATED(4);
-  else if (w == 8) MST_GATED(8);
-  else if (w == 16) MST_GATED(16);
-  else if (w == 32) MST_GATED(32);
-  else MST_GATED(64);
+  if (p.T < 16 / (int)sizeof(T)) MST_GATED(4, false, true);
+  else if (w == 4) MST_GATED(4, false, false);
+  else if (w == 8) MST_GATED(8, false, false);
+  else if (w == 16) MST_GATED(16, false, false);
+  else if (w == 32) MST_GATED(32, false, false);
+  else if (p.tiles == 1) MST_GATED(64, false, false);
+  else MST_GATED(64, true, false);
 #undef MST_GATED
 }
 

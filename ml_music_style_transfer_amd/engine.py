@@ -582,7 +582,7 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
     a_t = sigmoid(gate_t), h_t = a_t h_{t-1} + (1 - a_t) x_t for x, gate (B, C, T), both float32,
     bfloat16 or float16 and views with unit time stride (the halves of one layer's output) read in
     place. h0 (B, C): the state before the first frame (None: zeros); with reverse=True time runs
-    from the last frame to the first. lengths (B,): frames at or past a clip's length are not read,
+    from the last frame to the first. lengths (B,): frames at or past a clip's length are not used,
     give h = 0 and no gradient, and leave the state as it is.
 
     Returns (h, last): h (B, C, T) in x's type, last (B, C) float32, the state that the next chunk
