@@ -229,18 +229,21 @@ int mst_adam_clip_f32(float* const* p, const float* const* g, float* const* m, f
  * B on the device, taken into [0, T]): frames at or past lengths[b] are not used, leave the state
  * as it is and give h = 0. reverse != 0: t runs from the last frame down, h0 enters there.
  * h: (B, C, T) contiguous; last (B, C): the state after the last frame (the first when reversed).
- * carry: B * C * mst_gated_tiles(T) floats for the backward (nullable when that is 0). States are
+ * carry: B * C * mst_gated_tiles(T) floats for the backward (nullable when that is 0); workspace
+ * of mst_gated_workspace_size bytes (nullable when that is 0), for _fwd and _bwd alike. States are
  * float whatever the type. */
 int32_t mst_gated_tiles(int32_t T);
+size_t mst_gated_workspace_size(int32_t B, int32_t C, int32_t T);
 int mst_gated_fwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,
                   int64_t gc, const float* h0, const int32_t* lengths, int32_t B, int32_t C, int32_t T,
-                  int32_t reverse, void* h, float* last, float* carry, void* stream);
+                  int32_t reverse, void* h, float* last, float* carry, void* workspace, size_t ws_bytes,
+                  void* stream);
 /* Gradients of x, gate (contiguous (B, C, T), zero past the lengths) and h0 (nullable), given those
  * of h (gh: contiguous (B, C, T), nullable) and of last (glast: (B, C), nullable). */
 int mst_gated_bwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,
                   int64_t gc, const float* h0, const int32_t* lengths, const float* carry,
                   const void* gh, const float* glast, int32_t B, int32_t C, int32_t T, int32_t reverse,
-                  void* dx, void* dgate, float* dh0, void* stream);
+                  void* dx, void* dgate, float* dh0, void* workspace, size_t ws_bytes, void* stream);
 /* One frame: state (B, C) is updated in place and h (B, C) contiguous receives it; x, gate (B, C)
  * by batch stride, unit channel stride. */
 int mst_gated_step(int32_t type, const void* x, int64_t xb, const void* gate, int64_t gb, int32_t B,

@@ -91,12 +91,14 @@ SIGNATURES = {
                                     c_void_p, c_float, c_float, c_float, c_float, c_float, c_float,
                                     c_float, c_void_p, c_void_p]),
     "mst_gated_tiles": (c_int32, [c_int32]),
+    "mst_gated_workspace_size": (c_size_t, [c_int32, c_int32, c_int32]),
     "mst_gated_fwd": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                 c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
-                                c_void_p, c_void_p, c_void_p]),
+                                c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mst_gated_bwd": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
-                                c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
+                                c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                c_void_p]),
     "mst_gated_step": (c_int32, [c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32,
                                  c_void_p, c_void_p, c_void_p]),
     "mst_scale_f32": (c_int32, [c_void_p, c_int64, c_float, c_void_p]),

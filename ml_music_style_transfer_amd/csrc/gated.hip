@@ -36,6 +36,10 @@ struct Args {
   const float* glast;  // (B, C), nullable
   void *dx, *dgate;    // (B, C, T) contiguous
   float* dh0;          // (B, C), nullable
+  // A long axis with few rows: `segs` waves a row, each `span` tiles. Their maps, in the order of
+  // the pass, are composed first (maps, (rows, segs)); each wave enters with those before it.
+  float2* maps;
+  int32_t segs, span;
   int32_t C, T, tiles;
   uint32_t rows;
 };
@@ -286,23 +290,95 @@ __device__ __forceinline__ uint32_t group_id() {
   return W == 64 ? __builtin_amdgcn_readfirstlane(i) : i;
 }
 
-// W lanes a row; MULTI: more than one tile (W = 64); SHORT: rows shorter than a piece (W = 4)
+// The state that enters segment `seg`: `s` through the maps of the segments before it.
+__device__ __forceinline__ float enter(const Args& p, uint32_t row, int seg, float s) {
+  const float2* m = p.maps + (long long)row * p.segs;
+  const int lane = threadIdx.x & 63;
+  for (int i = 0; i < seg; i += 64) {
+    float2 v = make_float2(1.f, 0.f);
+    if (i + lane < seg) v = m[i + lane];
+    float At, Ht;
+    scan<64, false>(v.x, v.y, At, Ht);
+    s = fmaf(At, s, Ht);
+  }
+  return s;
+}
+
+// The map of every segment, of the forward pass or (BWD) of what is handed back, which runs against
+// it: the lanes' maps of a tile composed by the scan's total, the tiles' one after the other.
+template <typename T, bool REV, bool BWD>
+__global__ __launch_bounds__(256) void gated_maps_kernel(const Args p) {
+  const uint32_t id = group_id<64>();
+  const uint32_t row = id / (uint32_t)p.segs;
+  if (row >= p.rows) return;
+  constexpr bool DOWN = REV != BWD;  // the pass runs from the last tile to the first
+  const int lane = threadIdx.x & 63, seg = id % (uint32_t)p.segs;
+  const Row<T> r(p, row);
+  const int end = max(r.len, 16 / (int)sizeof(T));
+  const T* other = !BWD ? r.x : p.gh ? (const T*)p.gh + (long long)row * p.T : r.x;
+  const int i0 = seg * p.span, i1 = min(i0 + p.span, p.tiles);
+  int t = (DOWN ? p.tiles - 1 - i0 : i0) * kTile + lane * V;
+  struct Tile {
+    Raw<T, false> x, g;
+  } u, v;
+  u.x.load(other, t, end);
+  u.g.load(r.g, t, end);
+  float As = 1.f, Hs = 0.f;
+  int i = i0;
+  auto step = [&](Tile& tile, Tile& next) __attribute__((always_inline)) {
+    float b[V], g[V], a[V], c[V];
+    const int now = t;
+    t += DOWN ? -kTile : kTile;
+    next.x.load(other, t, end);
+    next.g.load(r.g, t, end);
+    if (now - lane * V >= r.len) return;
+    tile.x.settle(now, end);
+    tile.g.settle(now, end);
+#pragma unroll
+    for (int k = 0; k < V; ++k) b[k] = BWD && !p.gh ? 0.f : tile.x[k], g[k] = tile.g[k];
+    if (now + V > r.len) hold(r.len - now, g, b);
+    float A = 1.f, H = 0.f, At, Ht;
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+      const int k = DOWN ? V - 1 - q : q;
+      gate_of(g[k], a[k], c[k]);
+      H = BWD ? a[k] * (b[k] + H) : fmaf(a[k], H, c[k] * b[k]);
+      A *= a[k];
+    }
+    scan<64, DOWN>(A, H, At, Ht);
+    Hs = fmaf(At, Hs, Ht);
+    As *= At;
+  };
+  step(u, v);
+  while (++i < i1) {
+    step(v, u);
+    if (++i == i1) break;
+    step(u, v);
+  }
+  if (lane == 0) p.maps[id] = make_float2(As, Hs);
+}
+
+// W lanes a row; MULTI: more than one tile (W = 64), in p.segs segments; SHORT: rows shorter than a
+// piece (W = 4)
 template <typename T, int W, bool REV, bool MULTI, bool SHORT>
 __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
-  const uint32_t row = group_id<W>();
+  const uint32_t id = group_id<W>(), row = MULTI ? id / (uint32_t)p.segs : id;
   if (row >= p.rows) return;
+  const int seg = MULTI ? id % (uint32_t)p.segs : 0;
+  const int i0 = MULTI ? seg * p.span : 0, i1 = MULTI ? min(i0 + p.span, p.tiles) : 1;
   const int lane = threadIdx.x & (W - 1);
   const Row<T> r(p, row);
   const int end = SHORT ? p.T : max(r.len, 16 / (int)sizeof(T));
   T* h = (T*)p.h + (long long)row * p.T;
   float s = p.h0 ? p.h0[row] : 0.f;
-  int t = (MULTI && REV ? p.tiles - 1 : 0) * kTile + lane * V;
+  if (MULTI && seg > 0) s = enter(p, row, seg, s);
+  int t = (MULTI && REV ? p.tiles - 1 - i0 : i0) * kTile + lane * V;
   struct Tile {
     Raw<T, SHORT> x, g;
   } u, v;
   u.x.load(r.x, t, end);
   u.g.load(r.g, t, end);
-  int i = 0;
+  int i = i0;
   // one tile; the next one's loads go to registers of their own (copies would wait for them)
   auto step = [&](Tile& tile, Tile& next) __attribute__((always_inline)) {
     if (MULTI && lane == 0) p.carry[(long long)row * p.tiles + (REV ? p.tiles - 1 - i : i)] = s;
@@ -346,32 +422,35 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
     store(h, now, p.T, b);
   };
   step(u, v);
-  while (MULTI && ++i < p.tiles) {
+  while (MULTI && ++i < i1) {
     step(v, u);
-    if (++i == p.tiles) break;
+    if (++i == i1) break;
     step(u, v);
   }
-  if (lane == (W == 64 || REV ? 0 : W - 1)) p.last[row] = s;
+  if ((!MULTI || i1 == p.tiles) && lane == (W == 64 || REV ? 0 : W - 1)) p.last[row] = s;
 }
 
 template <typename T, int W, bool REV, bool MULTI, bool SHORT>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
-  const uint32_t row = group_id<W>();
+  const uint32_t id = group_id<W>(), row = MULTI ? id / (uint32_t)p.segs : id;
   if (row >= p.rows) return;
+  const int seg = MULTI ? id % (uint32_t)p.segs : 0;
+  const int i0 = MULTI ? seg * p.span : 0, i1 = MULTI ? min(i0 + p.span, p.tiles) : 1;
   const int lane = threadIdx.x & (W - 1);
   const Row<T> r(p, row);
   const int end = SHORT ? p.T : max(r.len, 16 / (int)sizeof(T));
   const T* gh = p.gh ? (const T*)p.gh + (long long)row * p.T : r.x;
   float s = p.glast ? p.glast[row] : 0.f;
   const float h0 = p.h0 ? p.h0[row] : 0.f;
-  int t = (MULTI && !REV ? p.tiles - 1 : 0) * kTile + lane * V;
+  if (MULTI && seg > 0) s = enter(p, row, seg, s);
+  int t = (MULTI && !REV ? p.tiles - 1 - i0 : i0) * kTile + lane * V;
   struct Tile {
     Raw<T, SHORT> x, g, d;
   } v, w;
   v.x.load(r.x, t, end);
   v.g.load(r.g, t, end);
   v.d.load(gh, t, end);
-  int i = 0;
+  int i = i0;
   auto step = [&](Tile& tile, Tile& next) __attribute__((always_inline)) {
     const float in = MULTI ? p.carry[(long long)row * p.tiles + (REV ? i : p.tiles - 1 - i)] : h0;
     float x[V], g[V], d[V], a[V], c[V];
@@ -436,12 +515,12 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
     store((T*)p.dgate + (long long)row * p.T, now, p.T, diff);
   };
   step(v, w);
-  while (MULTI && ++i < p.tiles) {
+  while (MULTI && ++i < i1) {
     step(w, v);
-    if (++i == p.tiles) break;
+    if (++i == i1) break;
     step(v, w);
   }
-  if (p.dh0 && lane == (W == 64 || !REV ? 0 : W - 1)) p.dh0[row] = s;
+  if (p.dh0 && (!MULTI || i1 == p.tiles) && lane == (W == 64 || !REV ? 0 : W - 1)) p.dh0[row] = s;
 }
 
 template <typename T>
@@ -468,10 +547,22 @@ int lanes_of(int32_t T) {
   return w;
 }
 
+// Tiles of a segment (all of them: one wave a row). A wave takes about 0.8 us a tile forward and 1.1
+// us backward whatever the others do, so few rows with a long axis leave the chip idle; segments
+// read x and gate (gate and gh) twice and cost a launch. Float32, forward + backward, one wave a row
+// -> segments: 128 rows of 50001 frames 76 + 104 -> 27 + 36 us, 512 of 60000 110 + 219 -> 109 + 176, but
+// 1024 of 8192 (16 tiles) 20 + 30 -> 31 + 43 and 300 of 3500 (7 tiles) 16 + 17 -> 22 + 23. 8192 waves fill
+// the chip's slots (2048 waves: 117 + 197 in the second case).
+int span_of(long long rows, int tiles) {
+  if (rows > 640 || tiles < 20) return tiles;
+  return (int)((rows * tiles + 8191) / 8192);
+}
+
 template <typename T, bool REV, bool BWD>
 void launch_w(const Args& p, hipStream_t st) {
   const int w = lanes_of(p.T);
-  const dim3 grid((unsigned)(((long long)p.rows * w + 255) / 256));
+  const dim3 grid((unsigned)(((long long)p.rows * p.segs * w + 255) / 256));
+  if (p.segs > 1) hipLaunchKernelGGL((gated_maps_kernel<T, REV, BWD>), grid, dim3(256), 0, st, p);
 #define MST_GATED(W_, MULTI, SHORT)                                                                        \
   do {                                                                                                     \
     if (BWD) hipLaunchKernelGGL((gated_bwd_kernel<T, W_, REV, MULTI, SHORT>), grid, dim3(256), 0, st, p);  \
@@ -485,6 +576,19 @@ void launch_w(const Args& p, hipStream_t st) {
   else if (p.tiles == 1) MST_GATED(64, false, false);
   else MST_GATED(64, true, false);
 #undef MST_GATED
+}
+
+int segs_of(long long rows, int tiles) {
+  const int span = span_of(rows, tiles);
+  return (tiles + span - 1) / span;
+}
+
+// the sizes of a call; false where the workspace is too small
+bool set_sizes(Args& p, int32_t B, int32_t C, int32_t T, void* workspace, size_t ws_bytes) {
+  p.C = C, p.T = T, p.tiles = tiles_of(T), p.rows = (uint32_t)B * (uint32_t)C;
+  p.span = span_of(p.rows, p.tiles), p.segs = segs_of(p.rows, p.tiles);
+  p.maps = (float2*)workspace;
+  return p.segs == 1 || (workspace && ws_bytes >= (size_t)p.rows * p.segs * sizeof(float2));
 }
 
 template <bool BWD>
@@ -507,29 +611,37 @@ extern "C" {
 
 int32_t mst_gated_tiles(int32_t T) { return T > kTile ? tiles_of(T) : 0; }
 
+size_t mst_gated_workspace_size(int32_t B, int32_t C, int32_t T) {
+  if (!good_shape(MST_F32, B, C, T)) return 0;
+  const long long rows = (long long)B * C;
+  const int segs = segs_of(rows, tiles_of(T));
+  return segs > 1 ? (size_t)rows * segs * sizeof(float2) : 0;
+}
+
 int mst_gated_fwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,
                   int64_t gc, const float* h0, const int32_t* lengths, int32_t B, int32_t C, int32_t T,
-                  int32_t reverse, void* h, float* last, float* carry, void* stream) {
+                  int32_t reverse, void* h, float* last, float* carry, void* workspace, size_t ws_bytes,
+                  void* stream) {
   MST_REQUIRE(good_shape(type, B, C, T) && x && gate && h && last);
   MST_REQUIRE(T <= kTile || carry);
   Args p = {};
   p.x = x, p.xb = xb, p.xc = xc, p.gate = gate, p.gb = gb, p.gc = gc;
   p.h0 = h0, p.len = lengths, p.h = h, p.last = last, p.carry = carry;
-  p.C = C, p.T = T, p.tiles = tiles_of(T), p.rows = (uint32_t)B * (uint32_t)C;
+  MST_REQUIRE(set_sizes(p, B, C, T, workspace, ws_bytes));
   return launch<false>(p, type, reverse, (hipStream_t)stream);
 }
 
 int mst_gated_bwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,
                   int64_t gc, const float* h0, const int32_t* lengths, const float* carry,
                   const void* gh, const float* glast, int32_t B, int32_t C, int32_t T, int32_t reverse,
-                  void* dx, void* dgate, float* dh0, void* stream) {
+                  void* dx, void* dgate, float* dh0, void* workspace, size_t ws_bytes, void* stream) {
   MST_REQUIRE(good_shape(type, B, C, T) && x && gate && dx && dgate);
   MST_REQUIRE(T <= kTile || carry);
   Args p = {};
   p.x = x, p.xb = xb, p.xc = xc, p.gate = gate, p.gb = gb, p.gc = gc;
   p.h0 = h0, p.len = lengths, p.carry = const_cast<float*>(carry);
   p.gh = gh, p.glast = glast, p.dx = dx, p.dgate = dgate, p.dh0 = dh0;
-  p.C = C, p.T = T, p.tiles = tiles_of(T), p.rows = (uint32_t)B * (uint32_t)C;
+  MST_REQUIRE(set_sizes(p, B, C, T, workspace, ws_bytes));
   return launch<true>(p, type, reverse, (hipStream_t)stream);
 }
 

@@ -536,9 +536,11 @@ def gated_fwd(x, gate, h0, lengths, reverse):
         return h, h0.clone() if h0 is not None else torch.zeros(B, C, device=dev), carry
     last = torch.empty(B, C, device=dev, dtype=torch.float32)
     with L.device_of(dev):
+        ws, nb = workspace(_lib().mst_gated_workspace_size(B, C, T), dev)
         L.check(_lib().mst_gated_fwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
                                      gate.stride(0), gate.stride(1), _p(h0), _p(lengths), B, C, T,
-                                     1 if reverse else 0, _p(h), _p(last), _p(carry), L.stream()),
+                                     1 if reverse else 0, _p(h), _p(last), _p(carry), _p(ws), nb,
+                                     L.stream()),
                 "gated_recurrence")
     return h, last, carry
 
@@ -557,10 +559,12 @@ def gated_bwd(gh, glast, x, gate, h0, lengths, carry, reverse):
         return dx, dgate, glast.clone() if glast is not None else torch.zeros(B, C, device=dev)
     dh0 = torch.empty(B, C, device=dev, dtype=torch.float32)
     with L.device_of(dev):
+        ws, nb = workspace(_lib().mst_gated_workspace_size(B, C, T), dev)
         L.check(_lib().mst_gated_bwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
                                      gate.stride(0), gate.stride(1), _p(h0), _p(lengths), _p(carry),
                                      _p(gh), _p(glast), B, C, T, 1 if reverse else 0, _p(dx),
-                                     _p(dgate), _p(dh0), L.stream()), "gated_recurrence_backward")
+                                     _p(dgate), _p(dh0), _p(ws), nb, L.stream()),
+                "gated_recurrence_backward")
     return dx, dgate, dh0
 
 

@@ -114,14 +114,14 @@ def test_c_entries_refuse():
     ok = dict(type=0, B=2, C=3, T=4, x=p, gate=p, h=p, last=p, carry=q)
     for change in (dict(type=3), dict(type=-1), dict(B=0), dict(C=0), dict(T=0), dict(T=2 ** 31 - 1),
                    dict(B=2 ** 16, C=2 ** 16), dict(x=q), dict(gate=q), dict(h=q), dict(last=q),
-                   dict(T=257, carry=q)):
+                   dict(T=513, carry=q)):
         a = dict(ok, **change)
         assert lib.mst_gated_fwd(a["type"], a["x"], 12, 4, a["gate"], 12, 4, None, None, a["B"], a["C"],
-                                 a["T"], 0, a["h"], a["last"], a["carry"], None) == L.MST_EINVAL, change
+                                 a["T"], 0, a["h"], a["last"], a["carry"], None, 0, None) == L.MST_EINVAL, change
         if "last" not in change:
             assert lib.mst_gated_bwd(a["type"], a["x"], 12, 4, a["gate"], 12, 4, None, None, a["carry"],
-                                     None, None, a["B"], a["C"], a["T"], 0, a["h"], p, None,
-                                     None) == L.MST_EINVAL, change
+                                     None, None, a["B"], a["C"], a["T"], 0, a["h"], p, None, None,
+                                     0, None) == L.MST_EINVAL, change
     for a in ((5, p, p, p, p, 2), (0, q, p, p, p, 2), (0, p, q, p, p, 2), (0, p, p, q, p, 2),
               (0, p, p, p, q, 2), (0, p, p, p, p, 0)):
         assert lib.mst_gated_step(a[0], a[1], 3, a[2], 3, a[5], 3, a[3], a[4], None) == L.MST_EINVAL
