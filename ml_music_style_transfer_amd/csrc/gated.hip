@@ -538,14 +538,14 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const T* __restrict__ x
   h[i] = (T)s;
 }
 
-int tiles_of(int32_t T) { return (T + kTile - 1) / kTile; }
-
 // lanes of a row: the fewest that hold it in one tile
 int lanes_of(int32_t T) {
   int w = 4;
   while (w < 64 && w * V < T) w *= 2;
   return w;
 }
+
+int tiles_of(int32_t T) { return (T + kTile - 1) / kTile; }
 
 // Tiles of a segment (all of them: one wave a row). A wave takes about 0.8 us a tile forward and 1.1
 // us backward whatever the others do, so few rows with a long axis leave the chip idle; segments
@@ -600,9 +600,10 @@ int launch(const Args& p, int type, int reverse, hipStream_t st) {
   return MST_OK;
 }
 
+// (a grid has fewer than 2^32 threads)
 bool good_shape(int32_t type, int32_t B, int32_t C, int32_t T) {
-  return type >= MST_F32 && type <= MST_F16 && B > 0 && C > 0 && T > 0 &&
-         (long long)B * C < (1ll << 31) && T <= 0x7fffffff - kTile;
+  return type >= MST_F32 && type <= MST_F16 && B > 0 && C > 0 && T > 0 && T <= 0x7fffffff - 2 * kTile &&
+         (long long)B * C < (1ll << 31) && (long long)B * C * lanes_of(T) < (1ll << 32) - 256;
 }
 
 }  // namespace

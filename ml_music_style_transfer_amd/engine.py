@@ -587,11 +587,48 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
 
     Returns (h, last): h (B, C, T) in x's type, last (B, C) float32, the state that the next chunk
     starts from. Differentiable in x, gate and h0; states are float32 inside."""
-    h, last, _ = torch.ops.mst.gated_recurrence(x, gate, h0, lengths, bool(reverse))
+    if not _eager(x, gate, h0):
+        h, last, _ = torch.ops.mst.gated_recurrence(x, gate, h0, lengths, bool(reverse))
+    elif torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
+                                      or (h0 is not None and h0.requires_grad)):
+        h, last = _GatedFn.apply(x, gate, h0, lengths, bool(reverse))
+    else:
+        h, last, _ = K.gated_fwd(x, gate, h0, lengths, reverse)
     return h, last
+
+
+def _eager(*ts):
+    """True for ordinary tensors that nothing traces or transforms: the kernels may then be called
+    without the dispatcher's layers, which cost more than a small call's kernel (a single frame
+    18 us against 8)."""
+    return (not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
+            and torch._C._functorch.peek_interpreter_stack() is None
+            and all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts))
+
+
+class _GatedFn(torch.autograd.Function):
+    """torch.ops.mst.gated_recurrence's registered backward as one autograd node."""
+
+    @staticmethod
+    def forward(ctx, x, gate, h0, lengths, reverse):
+        h, last, carry = K.gated_fwd(x, gate, h0, lengths, reverse)
+        ctx.save_for_backward(x, gate, h0, lengths, carry)
+        ctx.set_materialize_grads(False)
+        ctx.reverse = reverse
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_h, g_last):
+        x, gate, h0, lengths, carry = ctx.saved_tensors
+        dx, dgate, dh0 = K.gated_bwd(g_h, g_last, x, gate, h0, lengths, carry, ctx.reverse)
+        return dx, dgate, dh0.to(h0.dtype) if h0 is not None else None, None, None
 
 
 def gated_recurrence_step(x, gate, state):
     """One frame of gated_recurrence for serving: x, gate (B, C); state (B, C) float32 contiguous is
     updated in place and its new values are returned in x's type. Not differentiable."""
+    if _eager(x, gate, state) and not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
+                                                                    or state.requires_grad)):
+        return K.gated_step(x, gate, state)
     return torch.ops.mst.gated_recurrence_step(x, gate, state)

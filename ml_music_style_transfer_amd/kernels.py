@@ -14,6 +14,7 @@ offset implements crop_and_concat (model.py:71-78).
 """
 import ctypes
 import os
+from array import array
 
 import torch
 
@@ -395,26 +396,6 @@ def _is_dense(t):
     return t.is_contiguous() or t.permute(memory_order(t)).is_contiguous()
 
 
-def _grad_table(ts):
-    """(addresses, sizes, element types, count) of dense gradients, as host arrays."""
-    n = len(ts)
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]),
-            (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
-            (ctypes.c_int32 * n)(*[L.TYPES[t.dtype] for t in ts]), n)
-
-
-def _check_grads(ts, what):
-    dev = ts[0].device
-    for t in ts:
-        if t.layout != torch.strided or t.dtype not in L.TYPES:
-            raise TypeError(f"{what}: dense float32, bfloat16 or float16 gradients, got {t.dtype} "
-                            f"({t.layout})")
-        if not t.is_cuda:
-            raise RuntimeError(f"{what}: CUDA (HIP) tensors only; there is no CPU path")
-        if t.device != dev:
-            raise ValueError(f"{what}: gradients on one device, got {dev} and {t.device}")
-
-
 def check_max_norm(max_norm):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -422,34 +403,77 @@ def check_max_norm(max_norm):
     return max_norm
 
 
+def _address(a):
+    return a.buffer_info()[0]
+
+
+class GradTable:
+    """Gradients as the host arrays that mst_grad_norm and mst_grad_scale take (addresses, sizes,
+    element types). A gradient with gaps between its elements goes in as a dense copy, which is
+    copied back after a change."""
+
+    def __init__(self, ts, what, writes=False):
+        self.device = dev = ts[0].device
+        ptr, numel, types = [], [], []
+        self.copies = []
+        for t in ts:
+            code = L.TYPES.get(t.dtype)
+            if code is None or t.layout is not torch.strided:
+                raise TypeError(f"{what}: dense float32, bfloat16 or float16 gradients, got {t.dtype} "
+                                f"({t.layout})")
+            if t.device != dev:
+                raise ValueError(f"{what}: gradients on one device, got {dev} and {t.device}")
+            if not t.is_contiguous() and not _is_dense(t):
+                if writes and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                    raise ValueError(f"{what}: an expanded gradient holds several elements in one "
+                                     "place; clone it first")
+                d = t.contiguous()
+                self.copies.append((t, d))
+                t = d
+            ptr.append(t.data_ptr())
+            numel.append(t.numel())
+            types.append(code)
+        if not ts[0].is_cuda:
+            raise RuntimeError(f"{what}: CUDA (HIP) tensors only; there is no CPU path")
+        self.tensors, self.count = ts, len(ts)
+        self.arrays = (array("Q", ptr), array("q", numel), array("i", types))
+
+    def args(self):
+        return (*(_address(a) for a in self.arrays), self.count)
+
+    def norm(self, out=None):
+        dev, lib = self.device, _lib()
+        norm = torch.empty((), device=dev, dtype=torch.float32) if out is None else out
+        ws, nb = workspace(lib.mst_grad_norm_workspace_size(self.count), dev)
+        L.check(lib.mst_grad_norm(*self.args(), L.ptr(norm), L.ptr(ws), nb, L.stream()), "grad_norm")
+        return norm
+
+    def scale(self, norm, max_norm):
+        L.check(_lib().mst_grad_scale(*self.args(), L.ptr(norm), max_norm, L.stream()),
+                "clip_grad_norm_ (gradients that share memory?)")
+        torch.autograd.graph.increment_version(self.tensors)
+        for t, d in self.copies:
+            t.copy_(d)
+
+
 def grad_norm(ts, out=None):
     """L2 norm over every element of the tensors (0-d float32 on their device; sums in double, in
     an order that depends on the sizes alone), written to `out` if given."""
-    _check_grads(ts, "grad_norm")
-    dev = ts[0].device
-    with L.device_of(dev):
-        table = _grad_table([t if _is_dense(t) else t.contiguous() for t in ts])
-        norm = torch.empty((), device=dev, dtype=torch.float32) if out is None else out
-        lib = _lib()
-        ws, nb = workspace(lib.mst_grad_norm_workspace_size(table[3]), dev)
-        L.check(lib.mst_grad_norm(*table, L.ptr(norm), L.ptr(ws), nb, L.stream()), "grad_norm")
+    table = GradTable(ts, "grad_norm")
+    with L.device_of(table.device):
+        return table.norm(out)
+
+
+def clip_grad_norm_(ts, max_norm, check=None):
+    """g *= min(1, max_norm / (norm + 1e-6)) for every tensor, in place; returns the norm before.
+    check(norm), if given, runs before anything is changed."""
+    table = GradTable(ts, "clip_grad_norm_", writes=True)
+    with L.device_of(table.device):
+        norm = table.norm()
+        if check is not None:
+            check(norm)
+        table.scale(norm, max_norm)
     return norm
-
-
-def grad_scale_(ts, norm, max_norm):
-    """g *= min(1, max_norm / (norm + 1e-6)) for every tensor, in place; norm stays on the device."""
-    _check_grads(ts, "clip_grad_norm_")
-    for t in ts:
-        if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-            raise ValueError("clip_grad_norm_: an expanded gradient holds several elements in one "
-                             "place; clone it first")
-    with L.device_of(ts[0].device):
-        dense = [t if _is_dense(t) else t.contiguous() for t in ts]
-        L.check(_lib().mst_grad_scale(*_grad_table(dense), L.ptr(norm), max_norm, L.stream()),
-                "clip_grad_norm_ (gradients that share memory?)")
-        for t, d in zip(ts, dense):
-            if d is not t:
-                t.copy_(d)
 
 
 def adam_clip(ps, gs, ms, vs, norm, max_norm, lr_step, b1, b2, eps, bc2_sqrt, hyper=None):
@@ -458,19 +482,21 @@ def adam_clip(ps, gs, ms, vs, norm, max_norm, lr_step, b1, b2, eps, bc2_sqrt, hy
     n = len(ps)
     if not len(gs) == len(ms) == len(vs) == n:
         raise ValueError("adam_clip: as many gradients and moments as parameters")
-    for quad in zip(ps, gs, ms, vs):
-        for t in quad:
-            if t.dtype != torch.float32 or not t.is_cuda:
-                raise TypeError(f"adam_clip: float32 CUDA tensors, got {t.dtype} on {t.device}")
-            if t.numel() != quad[0].numel() or t.device != ps[0].device:
-                raise ValueError("adam_clip: sizes or devices differ")
     if n == 0:
         return
-    with L.device_of(ps[0].device):
-        arrays = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in (ps, gs, ms, vs)]
-        numel = (ctypes.c_int64 * n)(*[t.numel() for t in ps])
-        L.check(_lib().mst_adam_clip_f32(*arrays, numel, n, L.ptr(norm), max_norm, lr_step, b2,
-                                         1.0 - b1, 1.0 - b2, eps, bc2_sqrt, L.ptr(hyper), L.stream()),
+    dev, f32 = ps[0].device, torch.float32
+    for ts in (ps, gs, ms, vs):
+        for t in ts:
+            if t.dtype is not f32 or t.device != dev or not t.is_cuda:
+                raise TypeError(f"adam_clip: float32 CUDA tensors on one device, got {t.dtype} on {t.device}")
+    numel = [t.numel() for t in ps]
+    for ts in (gs, ms, vs):
+        if [t.numel() for t in ts] != numel:
+            raise ValueError("adam_clip: sizes differ")
+    with L.device_of(dev):
+        arrays = [array("Q", [t.data_ptr() for t in ts]) for ts in (ps, gs, ms, vs)] + [array("q", numel)]
+        L.check(_lib().mst_adam_clip_f32(*(_address(a) for a in arrays), n, L.ptr(norm), max_norm, lr_step,
+                                         b2, 1.0 - b1, 1.0 - b2, eps, bc2_sqrt, L.ptr(hyper), L.stream()),
                 "adam_clip (parameters or moments that share memory?)")
 
 
@@ -594,6 +620,7 @@ def gated_step(x, gate, state):
             L.check(_lib().mst_gated_step(L.TYPES[x.dtype], _p(x), x.stride(0), _p(gate),
                                           gate.stride(0), B, C, _p(state), _p(h), L.stream()),
                     "gated_recurrence_step")
+        torch.autograd.graph.increment_version(state)
     return h
 
 

@@ -226,6 +226,7 @@ class Adam(torch.optim.Optimizer):
         if not groups:
             return
         self.grad_norm = K.grad_norm(grads)
+        torch.autograd.graph.increment_version([p for _, params, _, _ in groups for p in params])
         for group, params, flat, st in groups:
             b1, b2 = group["betas"]
             lr, eps = group["lr"], group["eps"]
@@ -261,20 +262,18 @@ _memory_order = K.memory_order
 
 
 def _grads_of(parameters, what):
-    """(parameters, gradients) of those that have one; data-parallel averages have landed."""
+    """(flat-buffer owners, gradients) of the parameters that have one; data-parallel averages
+    have landed."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     params = [p for p in parameters if p.grad is not None]
-    if len({id(p) for p in params}) != len(params):
+    if len(set(map(id, params))) != len(params):
         raise ValueError(f"{what}: a parameter is listed twice")
-    for owner in {id(o): o for o in (_owner(p) for p in params) if o is not None}.values():
+    refs = {getattr(p, "_mst_flat_owner", None) for p in params}
+    owners = [o for o in (ref() for ref in refs if ref is not None) if o is not None]
+    for owner in owners:
         dp.finish_gradients(owner)
-    return params, [p.grad for p in params]
-
-
-def _owner(p):
-    ref = getattr(p, "_mst_flat_owner", None)
-    return ref() if ref is not None else None
+    return owners, [p.grad for p in params]
 
 
 @torch.no_grad()
@@ -295,19 +294,20 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if float(norm_type) != 2.0:
         raise ValueError(f"clip_grad_norm_: the L2 norm only (norm_type=2.0), got {norm_type}")
     max_norm = K.check_max_norm(max_norm)
-    params, grads = _grads_of(parameters, "clip_grad_norm_")
+    owners, grads = _grads_of(parameters, "clip_grad_norm_")
     if not grads:
         return torch.tensor(0.0)
-    for p in params:
-        hook = getattr(_owner(p), "_mst_adam", None)
+    for owner in owners:
+        hook = getattr(owner, "_mst_adam", None)
         if hook is not None and hook.active and hook.launched:
             raise RuntimeError("clip_grad_norm_: the update of these gradients ran inside backward "
                                "(Adam.overlap_backward)")
-    norm = K.grad_norm(grads)
-    if error_if_nonfinite and not math.isfinite(norm.item()):
+    return K.clip_grad_norm_(grads, max_norm, _finite if error_if_nonfinite else None)
+
+
+def _finite(norm):
+    if not math.isfinite(norm.item()):
         raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {norm.item()}")
-    K.grad_scale_(grads, norm, max_norm)
-    return norm
 
 
 def _adam_param(p, state, lr_step, b1, b2, eps, bc2_sqrt):
@@ -330,6 +330,8 @@ def _adam_views(p, state):
             y = torch.empty_like(p)
             y.copy_(x)
             state[key] = y
+    if p.is_contiguous() and p.grad.is_contiguous():
+        return p.data, p.grad, state["exp_avg"], state["exp_avg_sq"], []
     perm = _memory_order(p)
     pv = p.data.permute(perm)
     mv, vv = state["exp_avg"].permute(perm), state["exp_avg_sq"].permute(perm)

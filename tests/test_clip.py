@@ -112,7 +112,13 @@ def test_data_parallel_average_lands_first(monkeypatch):
     for p in ps:
         p._mst_flat_owner = weakref.ref(owner)
     monkeypatch.setattr(K, "grad_norm", lambda ts: log.append("norm") or torch.tensor(3.0))
-    monkeypatch.setattr(K, "grad_scale_", lambda *a: log.append("scale"))
+
+    def clip(ts, max_norm, check):
+        norm = K.grad_norm(ts)
+        if check is not None:
+            check(norm)
+        log.append("scale")
+    monkeypatch.setattr(K, "clip_grad_norm_", clip)
     T.grad_norm(ps)
     T.clip_grad_norm_(ps, 1.0)
     assert log == ["finish", "norm", "finish", "norm", "scale"]
