@@ -139,12 +139,14 @@ __global__ __launch_bounds__(256) void norm_final_kernel(const double* __restric
   if (threadIdx.x == 0) norm[0] = (float)sqrt(s);
 }
 
+// From the end to the start: what the norm read last is still in the 256 MB cache (90 M float32
+// gradients, norm and scale: 208 -> 167 us; 726 M: 1533 -> 1508 us).
 __global__ __launch_bounds__(256) void clip_scale_kernel(const Table tb, const float* __restrict__ norm,
                                                          float max_norm) {
   const float f = clip_factor(norm[0], max_norm);
   if (f == 1.f) return;  // under the limit: a product by one would give every value back
-  for (int c = blockIdx.x; c < tb.chunks; c += gridDim.x) {
-    const int i = find(tb, c);
+  for (int k = blockIdx.x; k < tb.chunks; k += gridDim.x) {
+    const int c = tb.chunks - 1 - k, i = find(tb, c);
     const long long at = (long long)(c - tb.first[i]) * kChunk;
     const int n = (int)min((long long)kChunk, tb.n[i] - at);
     const int type = tb.type[i];
