@@ -229,11 +229,11 @@ int mst_adam_clip_f32(float* const* p, const float* const* g, float* const* m, f
  * B on the device, taken into [0, T]): frames at or past lengths[b] are not used, leave the state
  * as it is and give h = 0. reverse != 0: t runs from the last frame down, h0 enters there.
  * h: (B, C, T) contiguous; last (B, C): the state after the last frame (the first when reversed).
- * carry: B * C * mst_gated_tiles(T) floats for the backward (nullable when that is 0); workspace
+ * carry: B * C * mst_gated_tiles(type, T) floats for the backward (nullable when that is 0); workspace
  * of mst_gated_workspace_size bytes (nullable when that is 0), for _fwd and _bwd alike. States are
  * float whatever the type. */
-int32_t mst_gated_tiles(int32_t T);
-size_t mst_gated_workspace_size(int32_t B, int32_t C, int32_t T);
+int32_t mst_gated_tiles(int32_t type, int32_t T);
+size_t mst_gated_workspace_size(int32_t type, int32_t B, int32_t C, int32_t T);
 int mst_gated_fwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,
                   int64_t gc, const float* h0, const int32_t* lengths, int32_t B, int32_t C, int32_t T,
                   int32_t reverse, void* h, float* last, float* carry, void* workspace, size_t ws_bytes,

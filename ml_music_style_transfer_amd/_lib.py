@@ -90,8 +90,8 @@ SIGNATURES = {
     "mst_adam_clip_f32": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
                                     c_void_p, c_float, c_float, c_float, c_float, c_float, c_float,
                                     c_float, c_void_p, c_void_p]),
-    "mst_gated_tiles": (c_int32, [c_int32]),
-    "mst_gated_workspace_size": (c_size_t, [c_int32, c_int32, c_int32]),
+    "mst_gated_tiles": (c_int32, [c_int32, c_int32]),
+    "mst_gated_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "mst_gated_fwd": (c_int32, [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                 c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),

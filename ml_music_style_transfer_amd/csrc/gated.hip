@@ -20,8 +20,11 @@
 
 namespace {
 
-constexpr int V = 8;           // frames of a lane
-constexpr int kTile = 64 * V;  // frames of a whole wave: the step of `carry`
+constexpr int kV = 8;           // frames of a lane
+// 16-bit rows that 16 frames a lane fit into one tile: (16, 4096, 860) bfloat16, two tiles -> one, 69 + 109
+// -> 63 + 107 us; not float32 ((16, 2048, 860): 63 + 112 -> 71 + 122, its loads no longer fill lines)
+constexpr int kWide = 16;
+constexpr int kTile = 64 * kV;  // frames of a wave in rows of several tiles: the step of `carry`
 
 struct Args {
   const void *x, *gate;  // (B, C, T) by batch and channel strides, unit time stride
@@ -55,7 +58,7 @@ template <> struct Piece<_Float16> { typedef _Float16 t __attribute__((ext_vecto
 // past `end` reads the last 16 bytes before it, and settle() moves what belongs to the lane down.
 // Frames past the clip hold anything. `end` is the clip's length, or P in a shorter clip: the row
 // has T >= P frames. SHORT: rows of T < P frames, read frame by frame.
-template <typename T, bool SHORT> struct Raw {
+template <typename T, int V, bool SHORT> struct Raw {
   static constexpr int P = 16 / sizeof(T), N = V / P;
   typename Piece<T>::t q[N];
 
@@ -101,7 +104,7 @@ template <typename T, bool SHORT> struct Raw {
   __device__ __forceinline__ float operator[](int k) const { return (float)q[k / P][k % P]; }
 };
 
-template <typename T>
+template <typename T, int V>
 __device__ __forceinline__ void store(T* row, int t, int end, const float (&v)[V]) {
   constexpr int P = 16 / sizeof(T);
 #pragma unroll
@@ -149,6 +152,7 @@ __device__ __forceinline__ void gate_of(float g, float& a, float& c) {
 }
 
 // frames from `n` on become the identity: an infinite gate holds the state, and x adds nothing
+template <int V>
 __device__ __forceinline__ void hold(int n, float (&g)[V], float (&x)[V]) {
 #pragma unroll
   for (int k = 0; k < V; ++k) {
@@ -156,6 +160,7 @@ __device__ __forceinline__ void hold(int n, float (&g)[V], float (&x)[V]) {
     x[k] = k < n ? x[k] : 0.f;
   }
 }
+template <int V>
 __device__ __forceinline__ void clear(int n, float (&v)[V]) {
 #pragma unroll
   for (int k = 0; k < V; ++k) v[k] = k < n ? v[k] : 0.f;
@@ -234,8 +239,10 @@ __device__ __forceinline__ void finish_scan(float& A, float& H, float& At, float
     At = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, A), DOWN ? 0 : 63));
     Ht = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, H), DOWN ? 0 : 63));
   }
-  A = dpp<DOWN ? kWaveShl1 : kWaveShr1>(1.f, A);
-  H = dpp<DOWN ? kWaveShl1 : kWaveShr1>(0.f, H);
+  if constexpr (W > 1) {
+    A = dpp<DOWN ? kWaveShl1 : kWaveShr1>(1.f, A);
+    H = dpp<DOWN ? kWaveShl1 : kWaveShr1>(0.f, H);
+  }
   if constexpr (W < 64)
     if ((threadIdx.x & (W - 1)) == (DOWN ? W - 1 : 0)) A = 1.f, H = 0.f;
 }
@@ -248,8 +255,8 @@ __device__ __forceinline__ void scan(float& A, float& H, float& At, float& Ht) {
   if constexpr (W >= 16) {
     levels16<DOWN>(A, H);
   } else {
-    level<W, DOWN, 1>(A, H);
-    level<W, DOWN, 2>(A, H);
+    if constexpr (W > 1) level<W, DOWN, 1>(A, H);
+    if constexpr (W > 2) level<W, DOWN, 2>(A, H);
     if constexpr (W > 4) level<W, DOWN, 4>(A, H);
   }
   finish_scan<W, DOWN>(A, H, At, Ht);
@@ -308,6 +315,7 @@ __device__ __forceinline__ float enter(const Args& p, uint32_t row, int seg, flo
 // it: the lanes' maps of a tile composed by the scan's total, the tiles' one after the other.
 template <typename T, bool REV, bool BWD>
 __global__ __launch_bounds__(256) void gated_maps_kernel(const Args p) {
+  constexpr int V = kV;
   const uint32_t id = group_id<64>();
   const uint32_t row = id / (uint32_t)p.segs;
   if (row >= p.rows) return;
@@ -319,7 +327,7 @@ __global__ __launch_bounds__(256) void gated_maps_kernel(const Args p) {
   const int i0 = seg * p.span, i1 = min(i0 + p.span, p.tiles);
   int t = (DOWN ? p.tiles - 1 - i0 : i0) * kTile + lane * V;
   struct Tile {
-    Raw<T, false> x, g;
+    Raw<T, kV, false> x, g;
   } u, v;
   u.x.load(other, t, end);
   u.g.load(r.g, t, end);
@@ -359,8 +367,8 @@ __global__ __launch_bounds__(256) void gated_maps_kernel(const Args p) {
 }
 
 // W lanes a row; MULTI: more than one tile (W = 64), in p.segs segments; SHORT: rows shorter than a
-// piece (W = 4)
-template <typename T, int W, bool REV, bool MULTI, bool SHORT>
+// piece (W = 1)
+template <typename T, int W, int V, bool REV, bool MULTI, bool SHORT>
 __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
   const uint32_t id = group_id<W>(), row = MULTI ? id / (uint32_t)p.segs : id;
   if (row >= p.rows) return;
@@ -374,7 +382,7 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
   if (MULTI && seg > 0) s = enter(p, row, seg, s);
   int t = (MULTI && REV ? p.tiles - 1 - i0 : i0) * kTile + lane * V;
   struct Tile {
-    Raw<T, SHORT> x, g;
+    Raw<T, V, SHORT> x, g;
   } u, v;
   u.x.load(r.x, t, end);
   u.g.load(r.g, t, end);
@@ -430,7 +438,7 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
   if ((!MULTI || i1 == p.tiles) && lane == (W == 64 || REV ? 0 : W - 1)) p.last[row] = s;
 }
 
-template <typename T, int W, bool REV, bool MULTI, bool SHORT>
+template <typename T, int W, int V, bool REV, bool MULTI, bool SHORT>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
   const uint32_t id = group_id<W>(), row = MULTI ? id / (uint32_t)p.segs : id;
   if (row >= p.rows) return;
@@ -445,7 +453,7 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
   if (MULTI && seg > 0) s = enter(p, row, seg, s);
   int t = (MULTI && !REV ? p.tiles - 1 - i0 : i0) * kTile + lane * V;
   struct Tile {
-    Raw<T, SHORT> x, g, d;
+    Raw<T, V, SHORT> x, g, d;
   } v, w;
   v.x.load(r.x, t, end);
   v.g.load(r.g, t, end);
@@ -540,12 +548,14 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const T* __restrict__ x
 
 // lanes of a row: the fewest that hold it in one tile
 int lanes_of(int32_t T) {
-  int w = 4;
-  while (w < 64 && w * V < T) w *= 2;
+  int w = 1;
+  while (w < 64 && w * kV < T) w *= 2;
   return w;
 }
 
-int tiles_of(int32_t T) { return (T + kTile - 1) / kTile; }
+int tiles_of(int32_t type, int32_t T) {
+  return T <= (type == MST_F32 ? kTile : 64 * kWide) ? 1 : (T + kTile - 1) / kTile;
+}
 
 // Tiles of a segment (all of them: one wave a row). A wave takes about 0.8 us a tile forward and 1.1
 // us backward whatever the others do, so few rows with a long axis leave the chip idle; segments
@@ -563,18 +573,21 @@ void launch_w(const Args& p, hipStream_t st) {
   const int w = lanes_of(p.T);
   const dim3 grid((unsigned)(((long long)p.rows * p.segs * w + 255) / 256));
   if (p.segs > 1) hipLaunchKernelGGL((gated_maps_kernel<T, REV, BWD>), grid, dim3(256), 0, st, p);
-#define MST_GATED(W_, MULTI, SHORT)                                                                        \
+#define MST_GATED(W_, V_, MULTI, SHORT)                                                                        \
   do {                                                                                                     \
-    if (BWD) hipLaunchKernelGGL((gated_bwd_kernel<T, W_, REV, MULTI, SHORT>), grid, dim3(256), 0, st, p);  \
-    else hipLaunchKernelGGL((gated_fwd_kernel<T, W_, REV, MULTI, SHORT>), grid, dim3(256), 0, st, p);      \
+    if (BWD) hipLaunchKernelGGL((gated_bwd_kernel<T, W_, V_, REV, MULTI, SHORT>), grid, dim3(256), 0, st, p);  \
+    else hipLaunchKernelGGL((gated_fwd_kernel<T, W_, V_, REV, MULTI, SHORT>), grid, dim3(256), 0, st, p);      \
   } while (0)
-  if (p.T < 16 / (int)sizeof(T)) MST_GATED(4, false, true);
-  else if (w == 4) MST_GATED(4, false, false);
-  else if (w == 8) MST_GATED(8, false, false);
-  else if (w == 16) MST_GATED(16, false, false);
-  else if (w == 32) MST_GATED(32, false, false);
-  else if (p.tiles == 1) MST_GATED(64, false, false);
-  else MST_GATED(64, true, false);
+  if (p.T < 16 / (int)sizeof(T)) MST_GATED(1, kV, false, true);
+  else if (w == 1) MST_GATED(1, kV, false, false);
+  else if (w == 2) MST_GATED(2, kV, false, false);
+  else if (w == 4) MST_GATED(4, kV, false, false);
+  else if (w == 8) MST_GATED(8, kV, false, false);
+  else if (w == 16) MST_GATED(16, kV, false, false);
+  else if (w == 32) MST_GATED(32, kV, false, false);
+  else if (p.T <= kTile) MST_GATED(64, kV, false, false);
+  else if (p.tiles > 1) MST_GATED(64, kV, true, false);
+  else if constexpr (sizeof(T) == 2) MST_GATED(64, kWide, false, false);
 #undef MST_GATED
 }
 
@@ -584,8 +597,8 @@ int segs_of(long long rows, int tiles) {
 }
 
 // the sizes of a call; false where the workspace is too small
-bool set_sizes(Args& p, int32_t B, int32_t C, int32_t T, void* workspace, size_t ws_bytes) {
-  p.C = C, p.T = T, p.tiles = tiles_of(T), p.rows = (uint32_t)B * (uint32_t)C;
+bool set_sizes(Args& p, int32_t type, int32_t B, int32_t C, int32_t T, void* workspace, size_t ws_bytes) {
+  p.C = C, p.T = T, p.tiles = tiles_of(type, T), p.rows = (uint32_t)B * (uint32_t)C;
   p.span = span_of(p.rows, p.tiles), p.segs = segs_of(p.rows, p.tiles);
   p.maps = (float2*)workspace;
   return p.segs == 1 || (workspace && ws_bytes >= (size_t)p.rows * p.segs * sizeof(float2));
@@ -610,12 +623,15 @@ bool good_shape(int32_t type, int32_t B, int32_t C, int32_t T) {
 
 extern "C" {
 
-int32_t mst_gated_tiles(int32_t T) { return T > kTile ? tiles_of(T) : 0; }
+int32_t mst_gated_tiles(int32_t type, int32_t T) {
+  const int tiles = tiles_of(type, T);
+  return tiles > 1 ? tiles : 0;
+}
 
-size_t mst_gated_workspace_size(int32_t B, int32_t C, int32_t T) {
-  if (!good_shape(MST_F32, B, C, T)) return 0;
+size_t mst_gated_workspace_size(int32_t type, int32_t B, int32_t C, int32_t T) {
+  if (!good_shape(type, B, C, T)) return 0;
   const long long rows = (long long)B * C;
-  const int segs = segs_of(rows, tiles_of(T));
+  const int segs = segs_of(rows, tiles_of(type, T));
   return segs > 1 ? (size_t)rows * segs * sizeof(float2) : 0;
 }
 
@@ -624,11 +640,11 @@ int mst_gated_fwd(int32_t type, const void* x, int64_t xb, int64_t xc, const voi
                   int32_t reverse, void* h, float* last, float* carry, void* workspace, size_t ws_bytes,
                   void* stream) {
   MST_REQUIRE(good_shape(type, B, C, T) && x && gate && h && last);
-  MST_REQUIRE(T <= kTile || carry);
+  MST_REQUIRE(tiles_of(type, T) == 1 || carry);
   Args p = {};
   p.x = x, p.xb = xb, p.xc = xc, p.gate = gate, p.gb = gb, p.gc = gc;
   p.h0 = h0, p.len = lengths, p.h = h, p.last = last, p.carry = carry;
-  MST_REQUIRE(set_sizes(p, B, C, T, workspace, ws_bytes));
+  MST_REQUIRE(set_sizes(p, type, B, C, T, workspace, ws_bytes));
   return launch<false>(p, type, reverse, (hipStream_t)stream);
 }
 
@@ -637,12 +653,12 @@ int mst_gated_bwd(int32_t type, const void* x, int64_t xb, int64_t xc, const voi
                   const void* gh, const float* glast, int32_t B, int32_t C, int32_t T, int32_t reverse,
                   void* dx, void* dgate, float* dh0, void* workspace, size_t ws_bytes, void* stream) {
   MST_REQUIRE(good_shape(type, B, C, T) && x && gate && dx && dgate);
-  MST_REQUIRE(T <= kTile || carry);
+  MST_REQUIRE(tiles_of(type, T) == 1 || carry);
   Args p = {};
   p.x = x, p.xb = xb, p.xc = xc, p.gate = gate, p.gb = gb, p.gc = gc;
   p.h0 = h0, p.len = lengths, p.carry = const_cast<float*>(carry);
   p.gh = gh, p.glast = glast, p.dx = dx, p.dgate = dgate, p.dh0 = dh0;
-  MST_REQUIRE(set_sizes(p, B, C, T, workspace, ws_bytes));
+  MST_REQUIRE(set_sizes(p, type, B, C, T, workspace, ws_bytes));
   return launch<true>(p, type, reverse, (hipStream_t)stream);
 }
 

@@ -501,11 +501,14 @@ def adam_clip(ps, gs, ms, vs, norm, max_norm, lr_step, b1, b2, eps, bc2_sqrt, hy
 
 
 # ---------------------------------------------------------- gated linear recurrence
-GATED_TILE = 512  # frames between two kept states (gated.hip; mst_gated_tiles)
+GATED_TILE = 512  # frames between two kept states (gated.hip)
 
 
-def gated_tiles(T):
-    return (T + GATED_TILE - 1) // GATED_TILE if T > GATED_TILE else 0
+def gated_tiles(dtype, T):
+    """States that the backward needs of a row of T frames (mst_gated_tiles): none in one tile, of
+    512 frames in float32 and up to 1024 in 16 bits."""
+    one = GATED_TILE if dtype == torch.float32 else 2 * GATED_TILE
+    return (T + GATED_TILE - 1) // GATED_TILE if T > one else 0
 
 
 def gated_check(x, gate, h0, lengths):
@@ -551,18 +554,18 @@ def _p(t):
 
 
 def gated_fwd(x, gate, h0, lengths, reverse):
-    """(h, last, carry) of mst_gated_fwd; carry (B, C, gated_tiles(T)) goes to gated_bwd."""
+    """(h, last, carry) of mst_gated_fwd; carry (B, C, gated_tiles(x.dtype, T)) goes to gated_bwd."""
     gated_check(x, gate, h0, lengths)
     x, gate, h0, lengths = _gated_inputs(x, gate, h0, lengths)
     B, C, T = x.shape
     dev = x.device
     h = torch.empty(B, C, T, device=dev, dtype=x.dtype)
-    carry = torch.empty(B, C, gated_tiles(T), device=dev, dtype=torch.float32)
+    carry = torch.empty(B, C, gated_tiles(x.dtype, T), device=dev, dtype=torch.float32)
     if h.numel() == 0:  # no frame: the state stays
         return h, h0.clone() if h0 is not None else torch.zeros(B, C, device=dev), carry
     last = torch.empty(B, C, device=dev, dtype=torch.float32)
     with L.device_of(dev):
-        ws, nb = workspace(_lib().mst_gated_workspace_size(B, C, T), dev)
+        ws, nb = workspace(_lib().mst_gated_workspace_size(L.TYPES[x.dtype], B, C, T), dev)
         L.check(_lib().mst_gated_fwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
                                      gate.stride(0), gate.stride(1), _p(h0), _p(lengths), B, C, T,
                                      1 if reverse else 0, _p(h), _p(last), _p(carry), _p(ws), nb,
@@ -585,7 +588,7 @@ def gated_bwd(gh, glast, x, gate, h0, lengths, carry, reverse):
         return dx, dgate, glast.clone() if glast is not None else torch.zeros(B, C, device=dev)
     dh0 = torch.empty(B, C, device=dev, dtype=torch.float32)
     with L.device_of(dev):
-        ws, nb = workspace(_lib().mst_gated_workspace_size(B, C, T), dev)
+        ws, nb = workspace(_lib().mst_gated_workspace_size(L.TYPES[x.dtype], B, C, T), dev)
         L.check(_lib().mst_gated_bwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
                                      gate.stride(0), gate.stride(1), _p(h0), _p(lengths), _p(carry),
                                      _p(gh), _p(glast), B, C, T, 1 if reverse else 0, _p(dx),

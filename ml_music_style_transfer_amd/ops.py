@@ -525,7 +525,7 @@ def _gated_fake(x, gate, h0, lengths, reverse):
     K.gated_check(x, gate, h0, lengths)
     B, C, T = x.shape
     return (x.new_empty(B, C, T), x.new_empty(B, C, dtype=torch.float32),
-            x.new_empty(B, C, K.gated_tiles(T), dtype=torch.float32))
+            x.new_empty(B, C, K.gated_tiles(x.dtype, T), dtype=torch.float32))
 
 
 @custom_op("mst::gated_recurrence_backward", mutates_args=())

@@ -63,13 +63,14 @@ def test_oracle_gradients(reverse):
 
 def test_fake_shapes_and_tiles():
     lib = L.load()
-    for T in (1, 255, 256, 257, 512, 513, 100000):
-        assert lib.mst_gated_tiles(T) == K.gated_tiles(T)
+    for T in (1, 512, 513, 1024, 1025, 100000):
+        for dtype, code in L.TYPES.items():
+            assert lib.mst_gated_tiles(code, T) == K.gated_tiles(dtype, T)
     with FakeTensorMode():
-        x = torch.empty(2, 5, 600, device="cuda", dtype=torch.bfloat16)
+        x = torch.empty(2, 5, 1600, device="cuda", dtype=torch.bfloat16)
         h, last, carry = torch.ops.mst.gated_recurrence(x, x, None, None, False)
         assert h.shape == x.shape and h.dtype == x.dtype
-        assert last.shape == (2, 5) and last.dtype == torch.float32 and carry.shape == (2, 5, K.gated_tiles(600))
+        assert last.shape == (2, 5) and last.dtype == torch.float32 and carry.shape == (2, 5, K.gated_tiles(x.dtype, 1600))
         dx, dg, dh0 = torch.ops.mst.gated_recurrence_backward(h, last, x, x, None, None, carry, False)
         assert dx.shape == dg.shape == x.shape and dh0.shape == (2, 5)
         s = torch.empty(2, 5, device="cuda")
@@ -114,7 +115,7 @@ def test_c_entries_refuse():
     ok = dict(type=0, B=2, C=3, T=4, x=p, gate=p, h=p, last=p, carry=q)
     for change in (dict(type=3), dict(type=-1), dict(B=0), dict(C=0), dict(T=0), dict(T=2 ** 31 - 1),
                    dict(B=2 ** 16, C=2 ** 16), dict(x=q), dict(gate=q), dict(h=q), dict(last=q),
-                   dict(T=513, carry=q)):
+                   dict(T=1025, carry=q)):
         a = dict(ok, **change)
         assert lib.mst_gated_fwd(a["type"], a["x"], 12, 4, a["gate"], 12, 4, None, None, a["B"], a["C"],
                                  a["T"], 0, a["h"], a["last"], a["carry"], None, 0, None) == L.MST_EINVAL, change
