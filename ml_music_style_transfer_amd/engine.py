@@ -585,6 +585,9 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
     from the last frame to the first. lengths (B,): frames at or past a clip's length are not used,
     give h = 0 and no gradient, and leave the state as it is.
 
+    A value or gate that is not finite makes the row's state that from its frame on; no frame before
+    it and no other row is touched.
+
     Returns (h, last): h (B, C, T) in x's type, last (B, C) float32, the state that the next chunk
     starts from. Differentiable in x, gate and h0; states are float32 inside."""
     if not _eager(x, gate, h0):

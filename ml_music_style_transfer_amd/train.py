@@ -55,6 +55,9 @@ class Adam(torch.optim.Optimizer):
     0-d device tensor; reading it waits for the device).
     """
 
+    max_norm = None
+    grad_norm = None
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0,
                  amsgrad=False, max_norm=None):
         if weight_decay != 0 or amsgrad:
@@ -62,7 +65,9 @@ class Adam(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=0, amsgrad=False))
         self._flat_groups = {}
         self.max_norm = None if max_norm is None else K.check_max_norm(max_norm)
-        self.grad_norm = None  # of the last step with a max_norm
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), max_norm=self.max_norm)  # copies and pickles clip too
 
     def _flat_of(self, group, params):
         """Return (flat_param, flat_grad, numel, offsets) if params tile one model's flat buffers."""
@@ -241,14 +246,17 @@ class Adam(torch.optim.Optimizer):
                         self._owner.flat_runs()], st["step"] + 1)
                 self._count_step(st, params)
                 continue
-            by_step, copied = {}, []
-            for p in params:
-                state = self.state[p]
+            states = [self.state[p] for p in params]
+            for p, state in zip(params, states):
                 if len(state) == 0 or state.get("exp_avg") is None:
                     state["step"] = torch.tensor(0.0)
                     state["exp_avg"] = torch.zeros_like(p)
                     state["exp_avg_sq"] = torch.zeros_like(p)
-                state["step"] += 1
+                elif not torch.is_tensor(state["step"]):  # a checkpoint that holds plain numbers
+                    state["step"] = torch.tensor(float(state["step"]))
+            torch._foreach_add_([state["step"] for state in states], 1.0)
+            by_step, copied = {}, []
+            for p, state in zip(params, states):
                 pv, g, mv, vv, back = _adam_views(p, state)
                 by_step.setdefault(float(state["step"]), []).append((pv, g, mv, vv))
                 copied += back

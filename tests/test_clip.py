@@ -60,6 +60,14 @@ def test_refusals():
         K.adam_clip([p], [p.grad], [p], [p], None, 1.0, 1e-3, 0.9, 0.999, 1e-8, 1.0)
 
 
+def test_copies_of_the_optimizer_clip():
+    import copy
+    import pickle
+    opt = T.Adam(_params([torch.ones(4)]), max_norm=0.5)
+    assert copy.deepcopy(opt).max_norm == 0.5 and pickle.loads(pickle.dumps(opt)).max_norm == 0.5
+    assert "max_norm" not in opt.state_dict()["param_groups"][0]  # torch.optim.Adam's format
+
+
 def test_c_entries_refuse():
     lib = L.load()
 
@@ -211,6 +219,33 @@ def test_views_and_orders(cuda):
     twice = _params([base[:10], base[5:15]])
     with pytest.raises(ValueError, match="share memory"):
         T.clip_grad_norm_(twice, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_slices_that_start_anywhere(cuda, dtype):
+    """Every start and length within a vector of 16 bytes, and what lies around stays as it was."""
+    base = torch.full((64, 64), 3.0, device=cuda, dtype=dtype)
+    vals = _grads([1 + (7 * i) % 40 for i in range(64)], [dtype], seed=8)
+    ps = _params([base[i, i % 9:i % 9 + v.numel()] for i, v in enumerate(vals)])
+    for p, v in zip(ps, vals):
+        p.grad.copy_(v)
+    ref = R.norm(vals)
+    _norm_ok(T.clip_grad_norm_(ps, ref / 5), ref)
+    rest = torch.ones_like(base, dtype=torch.bool)
+    for i, (p, v) in enumerate(zip(ps, vals)):
+        want, tol = R.scaled(v, R.factor(ref, ref / 5))
+        assert ((p.grad.cpu().double() - want).abs() <= tol).all()
+        rest[i, i % 9:i % 9 + v.numel()] = False
+    assert (base[rest] == 3.0).all()
+
+
+@pytest.mark.gpu
+def test_clip_counts_in_versions(cuda):
+    ps = _params([torch.ones(5, device=cuda)])
+    version = ps[0].grad._version
+    T.clip_grad_norm_(ps, 1.0)
+    assert ps[0].grad._version > version
 
 
 @pytest.mark.gpu

@@ -165,8 +165,8 @@ def _check(cuda, x, gate, gh, h0=None, gl=None, lengths=None, reverse=False, got
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("reverse", [False, True], ids=["fwd", "rev"])
-@pytest.mark.parametrize("T", [1, 2, 3, 5, 15, 16, 17, 31, 33, 64, 65, 127, 129, 252, 256, 257, 511, 513,
-                               1000, 2049])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 33, 64, 65, 127, 129, 252, 256, 257, 511, 512, 513,
+                               1000, 1024, 1025, 2049])
 def test_lengths_of_the_axis(cuda, T, reverse):
     x, gate, gh, h0, gl = _data(3, 7, T, seed=T)
     _check(cuda, x, gate, gh, h0, gl, None, reverse)
@@ -174,7 +174,7 @@ def test_lengths_of_the_axis(cuda, T, reverse):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
-@pytest.mark.parametrize("T", [1, 6, 63, 252, 257, 860])
+@pytest.mark.parametrize("T", [1, 6, 7, 8, 9, 17, 63, 252, 257, 513, 860, 1024, 1025])
 def test_types(cuda, T, dtype):
     x, gate, gh, h0, gl = _data(2, 5, T, dtype, seed=T + 1)
     for reverse in (False, True):
@@ -281,6 +281,12 @@ def test_extreme_gates_and_values(cuda, reverse):
         assert torch.equal(hb[4, :, before], h[4, :, before]) and torch.equal(hb[4, 1], h[4, 1])
         assert torch.equal(hb[:4], h[:4])
         assert not torch.isfinite(hb[4, 0, at])
+    gn = gate.clone()
+    gn[4, 0, at] = float("nan")
+    hb = E.gated_recurrence(x.to(cuda), gn.to(cuda), h0.to(cuda), None, reverse)[0]
+    assert torch.equal(hb[4, 0, before], h[4, 0, before]) and torch.equal(hb[4, 1], h[4, 1])
+    after = slice(0, at + 1) if reverse else slice(at, None)
+    assert hb[4, 0, after].isnan().all()
 
 
 def _replaced(gh, gl, reverse):
@@ -433,6 +439,33 @@ def test_step_captured(cuda):
         graph.replay()
         assert torch.equal(y, E.gated_recurrence_step(x[..., t].to(cuda), gate[..., t].to(cuda), e))
     assert torch.equal(s, e)
+
+
+@pytest.mark.gpu
+def test_operator_and_direct_call_agree(cuda):
+    """engine's direct calls and the registered operator are the same kernels; inference mode; the
+    in-place update counts in the state's version."""
+    x, gate, gh, h0, _ = (t.to(cuda) for t in _data(2, 5, 700, seed=15))
+    leaves = [t.clone().requires_grad_() for t in (x, gate, h0)]
+    want = torch.ops.mst.gated_recurrence(*leaves, None, True)
+    grads = torch.autograd.grad(want[0], leaves, gh)
+    h, last = E.gated_recurrence(*leaves, None, True)
+    assert torch.equal(h, want[0]) and torch.equal(last, want[1])
+    for a, b in zip(torch.autograd.grad(h, leaves, gh), grads):
+        assert torch.equal(a, b)
+    with torch.inference_mode():
+        h, last = E.gated_recurrence(x, gate, h0, None, True)
+        assert torch.equal(h, want[0]) and torch.equal(last, want[1])
+        s = h0.clone()
+        y = E.gated_recurrence_step(x[..., 0], gate[..., 0], s)
+    s2 = h0.clone()
+    version = s2._version
+    assert torch.equal(torch.ops.mst.gated_recurrence_step(x[..., 0], gate[..., 0], s2), y)
+    assert torch.equal(s, s2) and s2._version > version
+    s3 = h0.clone()
+    version = s3._version
+    E.gated_recurrence_step(x[..., 0], gate[..., 0], s3)
+    assert s3._version > version
 
 
 @pytest.mark.gpu
