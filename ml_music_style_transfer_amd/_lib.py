@@ -163,7 +163,7 @@ def check(rc, what=""):
 
 def stream():
     """The current device's current stream (the raw handle: torch.cuda.current_stream() builds a
-    Stream object, 3 us a launch)."""
+    Stream object every time)."""
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
