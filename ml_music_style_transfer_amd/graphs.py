@@ -137,7 +137,6 @@ class GraphedTrainStep:
             K.grad_norm([self.gf[o:o + n] for o, n in runs], out=self.norm)
             K.adam_clip(*([x[o:o + n] for o, n in runs] for x in (self.pf, self.gf, st["m"], st["v"])),
                         self.norm, self.max_norm, 0.0, self.b1, self.b2, self.eps, 1.0, self.hyper)
-            self.opt.grad_norm = self.norm
         self.loss.copy_(loss)
 
     def __call__(self, x_midi, x_audio, cond, target):
@@ -166,6 +165,8 @@ class GraphedTrainStep:
                 self._program(st)
             self._captured_st = st
             self.graph.replay()
+        if self.max_norm is not None:
+            self.opt.grad_norm = self.norm
         self.calls += 1
         self.opt._count_step(st, self.params)
         self._host_step = st["step"]

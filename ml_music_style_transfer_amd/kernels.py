@@ -413,30 +413,30 @@ class GradTable:
     copied back after a change."""
 
     def __init__(self, ts, what, writes=False):
+        # one property of all tensors at a time: a list of hundreds is bound by these loops
         self.device = dev = ts[0].device
-        ptr, numel, types = [], [], []
-        self.copies = []
-        for t in ts:
-            code = L.TYPES.get(t.dtype)
-            if code is None or t.layout is not torch.strided:
-                raise TypeError(f"{what}: dense float32, bfloat16 or float16 gradients, got {t.dtype} "
-                                f"({t.layout})")
-            if t.device != dev:
-                raise ValueError(f"{what}: gradients on one device, got {dev} and {t.device}")
-            if not t.is_contiguous() and not _is_dense(t):
-                if writes and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-                    raise ValueError(f"{what}: an expanded gradient holds several elements in one "
-                                     "place; clone it first")
-                d = t.contiguous()
-                self.copies.append((t, d))
-                t = d
-            ptr.append(t.data_ptr())
-            numel.append(t.numel())
-            types.append(code)
-        if not ts[0].is_cuda:
+        types = [L.TYPES.get(t.dtype) for t in ts]
+        if None in types or {t.layout for t in ts} != {torch.strided}:
+            bad = next(t for t in ts if t.dtype not in L.TYPES or t.layout != torch.strided)
+            raise TypeError(f"{what}: dense float32, bfloat16 or float16 gradients, got {bad.dtype} "
+                            f"({bad.layout})")
+        if not dev.type == "cuda":
             raise RuntimeError(f"{what}: CUDA (HIP) tensors only; there is no CPU path")
-        self.tensors, self.count = ts, len(ts)
-        self.arrays = (array("Q", ptr), array("q", numel), array("i", types))
+        if {t.get_device() for t in ts} != {dev.index}:
+            raise ValueError(f"{what}: gradients on one device, got {sorted({str(t.device) for t in ts})}")
+        self.tensors, self.count, self.copies = ts, len(ts), []
+        if not all([t.is_contiguous() for t in ts]):
+            ts = [t if _is_dense(t) else self._copy(t, what, writes) for t in ts]
+        self.arrays = (array("Q", [t.data_ptr() for t in ts]), array("q", [t.numel() for t in ts]),
+                       array("i", types))
+
+    def _copy(self, t, what, writes):
+        if writes and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{what}: an expanded gradient holds several elements in one place; clone it "
+                             "first")
+        d = t.contiguous()
+        self.copies.append((t, d))
+        return d
 
     def args(self):
         return (*(_address(a) for a in self.arrays), self.count)
@@ -484,13 +484,14 @@ def adam_clip(ps, gs, ms, vs, norm, max_norm, lr_step, b1, b2, eps, bc2_sqrt, hy
         raise ValueError("adam_clip: as many gradients and moments as parameters")
     if n == 0:
         return
-    dev, f32 = ps[0].device, torch.float32
-    for ts in (ps, gs, ms, vs):
-        for t in ts:
-            if t.dtype is not f32 or t.device != dev or not t.is_cuda:
-                raise TypeError(f"adam_clip: float32 CUDA tensors on one device, got {t.dtype} on {t.device}")
+    assert hyper is None or (hyper.dtype == torch.float32 and hyper.numel() >= 2 and hyper.is_cuda)
+    dev = ps[0].device
     numel = [t.numel() for t in ps]
-    for ts in (gs, ms, vs):
+    for ts in (ps, gs, ms, vs):
+        if {t.dtype for t in ts} != {torch.float32} or dev.type != "cuda" or \
+                {t.get_device() for t in ts} != {dev.index}:
+            raise TypeError("adam_clip: float32 CUDA tensors on one device, got "
+                            f"{sorted({f'{t.dtype} on {t.device}' for t in ts})}")
         if [t.numel() for t in ts] != numel:
             raise ValueError("adam_clip: sizes differ")
     with L.device_of(dev):
@@ -535,6 +536,21 @@ def gated_check(x, gate, h0, lengths):
             raise ValueError(f"gated_recurrence: tensors on one device, got {x.device} and {t.device}")
 
 
+def gated_bwd_check(gh, glast, x, gate, h0, lengths, carry):
+    gated_check(x, gate, h0, lengths)
+    B, C, T = x.shape
+    want = (B, C, gated_tiles(x.dtype, T))
+    if tuple(carry.shape) != want or carry.dtype != torch.float32 or not carry.is_contiguous():
+        raise ValueError(f"gated_recurrence_backward: carry must be the forward's, {want} float32, got "
+                         f"{tuple(carry.shape)} {carry.dtype}")
+    for t, shape in ((gh, (B, C, T)), (glast, (B, C))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"gated_recurrence_backward: a gradient of {shape}, got {tuple(t.shape)}")
+    for t in (gh, glast, carry):
+        if t is not None and t.device != x.device:
+            raise ValueError("gated_recurrence_backward: tensors on one device")
+
+
 def _unit_time(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
@@ -576,7 +592,7 @@ def gated_fwd(x, gate, h0, lengths, reverse):
 
 def gated_bwd(gh, glast, x, gate, h0, lengths, carry, reverse):
     """(dx, dgate, dh0) of mst_gated_bwd; gh and glast may be None (zeros)."""
-    gated_check(x, gate, h0, lengths)
+    gated_bwd_check(gh, glast, x, gate, h0, lengths, carry)
     x, gate, h0, lengths = _gated_inputs(x, gate, h0, lengths)
     B, C, T = x.shape
     dev = x.device

@@ -538,6 +538,7 @@ def gated_recurrence_backward(grad_h: Optional[Tensor], grad_last: Optional[Tens
 
 @gated_recurrence_backward.register_fake
 def _gated_bwd_fake(grad_h, grad_last, x, gate, h0, lengths, carry, reverse):
+    K.gated_bwd_check(grad_h, grad_last, x, gate, h0, lengths, carry)
     B, C, T = x.shape
     return x.new_empty(B, C, T), x.new_empty(B, C, T), x.new_empty(B, C, dtype=torch.float32)
 

@@ -274,14 +274,19 @@ def _grads_of(parameters, what):
     have landed."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    params = [p for p in parameters if p.grad is not None]
+    params, grads = [], []
+    for p in parameters:
+        g = p.grad
+        if g is not None:
+            params.append(p)
+            grads.append(g)
     if len(set(map(id, params))) != len(params):
         raise ValueError(f"{what}: a parameter is listed twice")
     refs = {getattr(p, "_mst_flat_owner", None) for p in params}
     owners = [o for o in (ref() for ref in refs if ref is not None) if o is not None]
     for owner in owners:
-        dp.finish_gradients(owner)
-    return owners, [p.grad for p in params]
+        dp.finish_gradients(owner)  # in place: the gradients stay the tensors that they are
+    return owners, grads
 
 
 @torch.no_grad()
@@ -332,14 +337,15 @@ def _adam_param(p, state, lr_step, b1, b2, eps, bc2_sqrt):
 def _adam_views(p, state):
     """(p, gradient, moments) of one parameter as dense tensors in p's memory order, and the
     [(destination, copy)] to write back after an update that ran on copies."""
+    m, v = state["exp_avg"], state["exp_avg_sq"]
+    if p.is_contiguous() and p.grad.is_contiguous() and m.is_contiguous() and v.is_contiguous():
+        return p, p.grad, m, v, []
     for key in ("exp_avg", "exp_avg_sq"):
         x = state[key]
         if x.stride() != p.stride():
             y = torch.empty_like(p)
             y.copy_(x)
             state[key] = y
-    if p.is_contiguous() and p.grad.is_contiguous():
-        return p.data, p.grad, state["exp_avg"], state["exp_avg_sq"], []
     perm = _memory_order(p)
     pv = p.data.permute(perm)
     mv, vv = state["exp_avg"].permute(perm), state["exp_avg_sq"].permute(perm)

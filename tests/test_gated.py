@@ -95,6 +95,13 @@ def test_refusals():
     for err, words, args in bad:
         with pytest.raises(err, match=words):
             E.gated_recurrence(*args)
+    x, back = z(2, 3, 2000), torch.ops.mst.gated_recurrence_backward
+    for gh, gl, carry, words in ((x, None, z(2, 3, 3), "carry must be"), (x, None, z(2, 4, 3).transpose(1, 2), "carry must be"),
+                                 (x, None, z(2, 3, 4, dtype=torch.float16), "carry must be"),
+                                 (z(2, 3, 1999), None, z(2, 3, 4), "a gradient of"),
+                                 (x, z(3, 2), z(2, 3, 4), "a gradient of")):
+        with pytest.raises(ValueError, match=words):
+            back(gh, gl, x, x, None, None, carry, False)
     for err, words, args in [
             (ValueError, "one shape", (z(2, 3), z(2, 3), z(3, 2))),
             (TypeError, "both float32", (z(2, 3), z(2, 3, dtype=torch.float16), z(2, 3))),
