@@ -19,8 +19,8 @@
 //
 // Bound by HBM in float32: (32, 1024, 252) takes 17 us forward and 27 us backward, 5.9 and 6.2 TB/s
 // of the 3 and 5 tensors that have to move. In 16 bits also by the vector unit's issue: a frame
-// costs some 24 instructions forward and 40 backward (14 of them its gate), and (16, 4096, 860) in
-// bfloat16 runs at 5.5 and 5.3 TB/s with three quarters of the issue slots taken. Rows of an odd
+// costs some 28 instructions forward and 43 backward (14 of them its gate), and (16, 4096, 860) in
+// bfloat16 runs at 5.5 and 5.3 TB/s with 93 % and 84 % of the issue slots taken. Rows of an odd
 // number of 16-bit frames, which start off any alignment, are the slowest ((64, 8192, 63) backward 84 us,
 // 3.9 TB/s).
 #include "common.h"

@@ -624,8 +624,9 @@ class _GatedFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_h, g_last):
         x, gate, h0, lengths, carry = ctx.saved_tensors
-        dx, dgate, dh0 = K.gated_bwd(g_h, g_last, x, gate, h0, lengths, carry, ctx.reverse)
-        return dx, dgate, dh0.to(h0.dtype) if h0 is not None else None, None, None
+        need = ctx.needs_input_grad[2]
+        dx, dgate, dh0 = K.gated_bwd(g_h, g_last, x, gate, h0, lengths, carry, ctx.reverse, need)
+        return dx, dgate, dh0.to(h0.dtype) if need else None, None, None
 
 
 def gated_recurrence_step(x, gate, state):

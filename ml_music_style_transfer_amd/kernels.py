@@ -565,6 +565,12 @@ def _gated_inputs(x, gate, h0, lengths):
     return _unit_time(x), _unit_time(gate), h0.float().contiguous() if h0 is not None else None, lengths
 
 
+def _gated_workspace(x, carry):
+    if carry.numel() == 0:  # rows of one tile need none
+        return None, 0
+    return workspace(_lib().mst_gated_workspace_size(L.TYPES[x.dtype], *x.shape), x.device)
+
+
 def _p(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
@@ -581,7 +587,7 @@ def gated_fwd(x, gate, h0, lengths, reverse):
         return h, h0.clone() if h0 is not None else torch.zeros(B, C, device=dev), carry
     last = torch.empty(B, C, device=dev, dtype=torch.float32)
     with L.device_of(dev):
-        ws, nb = workspace(_lib().mst_gated_workspace_size(L.TYPES[x.dtype], B, C, T), dev)
+        ws, nb = _gated_workspace(x, carry)
         L.check(_lib().mst_gated_fwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
                                      gate.stride(0), gate.stride(1), _p(h0), _p(lengths), B, C, T,
                                      1 if reverse else 0, _p(h), _p(last), _p(carry), _p(ws), nb,
@@ -590,8 +596,8 @@ def gated_fwd(x, gate, h0, lengths, reverse):
     return h, last, carry
 
 
-def gated_bwd(gh, glast, x, gate, h0, lengths, carry, reverse):
-    """(dx, dgate, dh0) of mst_gated_bwd; gh and glast may be None (zeros)."""
+def gated_bwd(gh, glast, x, gate, h0, lengths, carry, reverse, need_dh0=True):
+    """(dx, dgate, dh0) of mst_gated_bwd; gh and glast may be None (zeros), dh0 is None if not needed."""
     gated_bwd_check(gh, glast, x, gate, h0, lengths, carry)
     x, gate, h0, lengths = _gated_inputs(x, gate, h0, lengths)
     B, C, T = x.shape
@@ -602,9 +608,9 @@ def gated_bwd(gh, glast, x, gate, h0, lengths, carry, reverse):
     glast = glast.float().contiguous() if glast is not None else None
     if dx.numel() == 0:
         return dx, dgate, glast.clone() if glast is not None else torch.zeros(B, C, device=dev)
-    dh0 = torch.empty(B, C, device=dev, dtype=torch.float32)
+    dh0 = torch.empty(B, C, device=dev, dtype=torch.float32) if need_dh0 else None
     with L.device_of(dev):
-        ws, nb = workspace(_lib().mst_gated_workspace_size(L.TYPES[x.dtype], B, C, T), dev)
+        ws, nb = _gated_workspace(x, carry)
         L.check(_lib().mst_gated_bwd(L.TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(gate),
                                      gate.stride(0), gate.stride(1), _p(h0), _p(lengths), _p(carry),
                                      _p(gh), _p(glast), B, C, T, 1 if reverse else 0, _p(dx),
