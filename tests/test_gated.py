@@ -476,6 +476,32 @@ def test_operator_and_direct_call_agree(cuda):
 
 
 @pytest.mark.gpu
+def test_traced_and_differentiated_twice(cuda):
+    """A traced call goes through the registered operators and gives the direct call's values; a
+    second derivative is refused."""
+    x, gate, _, h0, _ = (t.to(cuda) for t in _data(2, 5, 700, seed=16))
+
+    def value(x, gate, h0):
+        h, last = E.gated_recurrence(x, gate, h0, None, True)
+        return (h * h).sum() + last.sum()
+
+    def frame(x, gate, state):
+        return E.gated_recurrence_step(x, gate, state) + 1
+    a, b = ([t.clone().requires_grad_() for t in (x, gate, h0)] for _ in range(2))
+    value(*a).backward()
+    torch.compile(value, backend="aot_eager", fullgraph=True)(*b).backward()
+    for u, v in zip(a, b):
+        assert torch.equal(u.grad, v.grad)
+    s, t = h0.clone(), h0.clone()
+    with torch.no_grad():
+        y = torch.compile(frame, backend="aot_eager", fullgraph=True)(x[..., 0], gate[..., 0], t)
+        assert torch.equal(frame(x[..., 0], gate[..., 0], s), y) and torch.equal(s, t)
+    grads = torch.autograd.grad(value(*a), a, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grads[0].sum().backward()
+
+
+@pytest.mark.gpu
 def test_opcheck(cuda):
     x, gate, _, h0, _ = _data(2, 3, 300, seed=14)
     args = (x.to(cuda).requires_grad_(), gate.to(cuda).requires_grad_(), h0.to(cuda).requires_grad_(),
