@@ -304,15 +304,18 @@ def _replaced(gh, gl, reverse):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,C,T", [(1, 1, 20011), (1, 3, 5000), (2, 40, 3001), (1, 300, 1500)])
-def test_few_rows_long_axis(cuda, B, C, T):
-    for k, dtype in enumerate((torch.float32, torch.bfloat16)):
-        x, gate, gh, h0, gl = _data(B, C, T, dtype, seed=T + k, shift=3.0)
-        for reverse in (False, True):
-            _check(cuda, x, gate, gh, h0, gl, None, reverse)
-    n = torch.tensor([T // 3] * B, dtype=torch.int32)
-    _check(cuda, x, gate, gh, h0, gl, n, False)
-    _check(cuda, x, gate, gh, h0, gl, n, True)
+@pytest.mark.parametrize("B,C,T,dtype,reverse,padded", [
+    (1, 2, 33501, torch.float32, False, False),   # 66 segments of one tile
+    (1, 2, 33501, torch.bfloat16, True, False),
+    (2, 250, 10301, torch.float32, True, True),   # segments of two tiles, the last of one
+    (2, 40, 10301, torch.float16, False, True),
+    (1, 3, 5000, torch.float16, True, True),      # one wave a row
+    (3, 100, 3001, torch.float32, False, False),
+    (1, 300, 1500, torch.bfloat16, True, True)])
+def test_long_axis(cuda, B, C, T, dtype, reverse, padded):
+    x, gate, gh, h0, gl = _data(B, C, T, dtype, seed=T, shift=3.0)
+    n = torch.tensor([T - 700, T // 3][:B], dtype=torch.int32) if padded else None
+    _check(cuda, x, gate, gh, h0, gl, n, reverse)
 
 
 @pytest.mark.gpu
