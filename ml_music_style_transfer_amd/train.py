@@ -70,13 +70,11 @@ class Adam(torch.optim.Optimizer):
         return dict(super().__getstate__(), max_norm=self.max_norm)  # copies and pickles clip too
 
     def _flat_of(self, group, params):
-        """Return (flat_param, flat_grad, numel, offsets) if params tile one model's flat buffers."""
-        ref = getattr(params[0], "_mst_flat_owner", None)
-        owner = ref() if ref is not None else getattr(self, "_owner", None)
+        """Return (flat_param, flat_grad, owner) if params tile one model's flat buffers."""
+        owner = self._owner_of(params)
         if owner is None or not owner._flat_ok():
             return None
-        self._owner = owner
-        pf, gf, n = owner.flat_buffers()
+        pf, gf, _ = owner.flat_buffers()
         index = owner._flat["index"]
         if len(params) != len(index):
             return None
@@ -88,7 +86,14 @@ class Adam(torch.optim.Optimizer):
             o = ent[0]
             if p.data_ptr() != base_p + 4 * o or p.grad.data_ptr() != base_g + 4 * o:
                 return None
-        return pf, gf, n
+        self._owner = owner
+        return pf, gf, owner
+
+    def _owner_of(self, params):
+        """The model whose flat buffers the parameters live in: the one that they name, or the
+        attached one. Groups may belong to different models."""
+        ref = getattr(params[0], "_mst_flat_owner", None)
+        return ref() if ref is not None else getattr(self, "_owner", None)
 
     def attach(self, model):
         """Declare the PerformanceNet whose flat buffers the parameters live in."""
@@ -126,7 +131,7 @@ class Adam(torch.optim.Optimizer):
             m = torch.zeros_like(pf)
             v = torch.zeros_like(pf)
             st = {"m": m, "v": v, "step": int(steps.pop()) if steps else 0}
-            index = self._owner._flat["index"]
+            index = self._owner_of(params)._flat["index"]
             for p in params:
                 o, k = index[id(p)]
                 mv, vv = slot_view(m[o:o + k], p), slot_view(v[o:o + k], p)
@@ -190,7 +195,7 @@ class Adam(torch.optim.Optimizer):
             flat = self._flat_of(group, params)
             st = self._flat_state(gi, flat[0], params) if flat is not None else None
             if st is not None:
-                pf, gf, n = flat
+                pf, gf, _ = flat
                 t = st["step"] + 1
                 bc1 = 1 - b1 ** t
                 bc2 = 1 - b2 ** t
@@ -222,7 +227,7 @@ class Adam(torch.optim.Optimizer):
             flat = self._flat_of(group, params)
             st = self._flat_state(gi, flat[0], params) if flat is not None else None
             if st is not None:
-                grads += [flat[1][o:o + n] for o, n in self._owner.flat_runs()]
+                grads += [flat[1][o:o + n] for o, n in flat[2].flat_runs()]
             else:
                 grads += [p.grad for p in params]
             if any(t.dtype != torch.float32 for p in params for t in (p, p.grad)):
@@ -241,9 +246,9 @@ class Adam(torch.optim.Optimizer):
                             eps, math.sqrt(1 - b2 ** t))
 
             if st is not None:
-                pf, gf, _ = flat
+                pf, gf, owner = flat
                 update([[x[o:o + n] for x in (pf, gf, st["m"], st["v"])] for o, n in
-                        self._owner.flat_runs()], st["step"] + 1)
+                        owner.flat_runs()], st["step"] + 1)
                 self._count_step(st, params)
                 continue
             states = [self.state[p] for p in params]
