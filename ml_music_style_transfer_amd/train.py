@@ -175,10 +175,12 @@ class Adam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        owner = getattr(self, "_owner", None)
-        reducer = getattr(owner, "_mst_dp", None) if owner is not None else None
-        if reducer is not None:
-            reducer.finish()  # overlapped data-parallel all-reduce must land first
+        attached = getattr(self, "_owner", None)
+        if attached is not None:
+            dp.finish_gradients(attached)  # overlapped data-parallel all-reduces must land first
+        for owner in _owners(p for group in self.param_groups for p in group["params"]):
+            if owner is not attached:
+                dp.finish_gradients(owner)
         bwd = getattr(self, "_bwd", None)
         if bwd is not None and bwd.finish():  # the update already ran inside backward
             self._count_step(bwd.st, bwd.params)
@@ -272,6 +274,12 @@ class Adam(torch.optim.Optimizer):
 
 
 _memory_order = K.memory_order
+
+
+def _owners(params):
+    """The models whose flat buffers the parameters live in, in the parameters' order."""
+    refs = {id(ref): ref for ref in (getattr(p, "_mst_flat_owner", None) for p in params) if ref is not None}
+    return [owner for owner in (ref() for ref in refs.values()) if owner is not None]
 
 
 def _grads_of(parameters, what):

@@ -60,3 +60,42 @@ def test_a_model_that_does_not_match_is_not_kept(kernels):
     opt.step()
     assert opt._owner is a
     assert all((p == -1).all() for p in (*a.w, b.w[0])) and (b.w[1] == 0).all()
+
+
+class _Average:
+    """A data-parallel average that is under way: it lands in finish()."""
+
+    def __init__(self, net):
+        self.net, self.finished = net, 0
+
+    def finish(self):
+        self.finished += 1
+        self.net._flat["grad"].mul_(0.5)
+
+
+@pytest.mark.parametrize("max_norm", [1.0, None])
+def test_average_lands_before_the_first_step(kernels, max_norm):
+    """An optimizer that no model was attached to, over two models and a parameter of none: the norm and
+    the update see the averaged gradients from the first step on."""
+    nets = [_Net(5, 3), _Net(7)]
+    for net in nets:
+        net._mst_dp = _Average(net)
+    free = nn.Parameter(torch.zeros(4))
+    free.grad = torch.ones(4)
+    opt = T.Adam([{"params": nets[0].parameters()}, {"params": nets[1].parameters()}, {"params": [free]}],
+                 max_norm=max_norm)
+    opt.step()
+    assert [net._mst_dp.finished for net in nets] == [1, 1]
+    assert all((p == -0.5).all() for net in nets for p in net.parameters()) and (free == -1).all()
+    if max_norm is not None:
+        assert opt.grad_norm.item() == pytest.approx((15 * 0.25 + 4) ** 0.5)
+
+
+def test_average_of_an_attached_model_lands(kernels):
+    """also where its parameters name no owner"""
+    net = _Net(5, 3)
+    net._mst_dp = _Average(net)
+    for p in net.w:
+        del p._mst_flat_owner
+    T.Adam(net.parameters(), max_norm=1.0).attach(net).step()
+    assert net._mst_dp.finished == 1 and all((p == -0.5).all() for p in net.w)
