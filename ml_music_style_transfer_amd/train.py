@@ -295,8 +295,7 @@ def _grads_of(parameters, what):
             grads.append(g)
     if len(set(map(id, params))) != len(params):
         raise ValueError(f"{what}: a parameter is listed twice")
-    refs = {getattr(p, "_mst_flat_owner", None) for p in params}
-    owners = [o for o in (ref() for ref in refs if ref is not None) if o is not None]
+    owners = _owners(params)
     for owner in owners:
         dp.finish_gradients(owner)  # in place: the gradients stay the tensors that they are
     return owners, grads

@@ -99,3 +99,16 @@ def test_average_of_an_attached_model_lands(kernels):
         del p._mst_flat_owner
     T.Adam(net.parameters(), max_norm=1.0).attach(net).step()
     assert net._mst_dp.finished == 1 and all((p == -0.5).all() for p in net.w)
+
+
+def test_parameters_that_outlive_their_model(monkeypatch):
+    """The norm and the clip over parameters whose model is gone."""
+    import gc
+    net = _Net(5, 3)
+    params = list(net.w)
+    del net
+    gc.collect()
+    monkeypatch.setattr(K, "grad_norm", lambda ts: torch.cat([t.flatten() for t in ts]).norm())
+    monkeypatch.setattr(K, "clip_grad_norm_", lambda ts, max_norm, check: K.grad_norm(ts))
+    assert T.grad_norm(params).item() == pytest.approx(8 ** 0.5)
+    assert T.clip_grad_norm_(params, 1.0).item() == pytest.approx(8 ** 0.5)
