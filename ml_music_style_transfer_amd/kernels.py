@@ -14,6 +14,7 @@ offset implements crop_and_concat (model.py:71-78).
 """
 import ctypes
 import os
+import threading
 from array import array
 
 import torch
@@ -70,15 +71,22 @@ def _dst(spec):
     return d
 
 
-# Workspace arena: one grow-only scratch buffer per (device, launch stream). Launches on one
-# stream are ordered, so consecutive GEMM split-K slabs and loss partials share it instead of
-# paying an allocator round trip each. An outgrown buffer is simply dropped: torch's caching
+# Workspace arena: one grow-only scratch buffer per (host thread, device, launch stream). Launches on
+# one stream are ordered, so consecutive GEMM split-K slabs and loss partials share it instead of
+# paying an allocator round trip each. Threads do not share: the launches of one call leave data for
+# each other there, and another thread's launches may come between them (autograd's thread has its
+# own, so a training step holds two). An outgrown buffer is simply dropped: torch's caching
 # allocator hands its block out again only in this stream's order, after the launches already
 # queued on it. Under stream capture the arena is bypassed (each launch takes a fresh buffer
 # from the graph's private pool, torch's capture semantics), so no graph names an arena
 # buffer. Requests above ARENA_MAX_BYTES (Griffin-Lim's multi-GB clip chunks) are one-off
 # allocations that return to the allocator after the call instead of staying pinned here.
-_ARENA = {}
+class _Arena(threading.local):
+    def __init__(self):
+        self.buffers = {}
+
+
+_ARENA = _Arena()
 ARENA_MAX_BYTES = 256 << 20
 
 
@@ -89,13 +97,13 @@ def workspace(nbytes, device):
     n = (nbytes + 3) // 4
     if torch.cuda.is_current_stream_capturing() or nbytes > ARENA_MAX_BYTES:
         return torch.empty(n, device=device, dtype=torch.float32), 4 * n
-    key = (device.index, L.stream().value)
-    buf = _ARENA.get(key)
+    key, arena = (device.index, L.stream().value), _ARENA.buffers
+    buf = arena.get(key)
     if buf is None or buf.numel() < n:
         if buf is not None:
             n = min(max(n, 2 * buf.numel()), ARENA_MAX_BYTES // 4)
-        _ARENA[key] = None  # release the outgrown block before taking the larger one
-        buf = _ARENA[key] = torch.empty(n, device=device, dtype=torch.float32)
+        arena[key] = None  # release the outgrown block before taking the larger one
+        buf = arena[key] = torch.empty(n, device=device, dtype=torch.float32)
     return buf, 4 * buf.numel()
 
 
