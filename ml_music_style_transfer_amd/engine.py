@@ -589,9 +589,10 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
     it and no other row is touched.
 
     Returns (h, last): h (B, C, T) in x's type, last (B, C) float32, the state that the next chunk
-    starts from. Differentiable in x, gate and h0; states are float32 inside."""
+    starts from. Differentiable in x, gate and h0, in reverse mode, once; states are float32 inside."""
+    K.refuse_tangents("gated_recurrence", x, gate, h0)
     if not _eager(x, gate, h0):
-        h, last, _ = torch.ops.mst.gated_recurrence(x, gate, h0, lengths, bool(reverse))
+        h, last, _ = _op(torch.ops.mst.gated_recurrence, x, gate, h0, lengths, bool(reverse))
     elif torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
                                       or (h0 is not None and h0.requires_grad)):
         h, last = _GatedFn.apply(x, gate, h0, lengths, bool(reverse))
@@ -609,6 +610,15 @@ def _eager(*ts):
             and all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts))
 
 
+def _op(op, *args):
+    """The registered operator on inputs without tangents. Inside forward mode it cannot tell (it sees
+    none of torch.func.jvp's tangents) and refuses, unless forward mode is off around it."""
+    if not K.in_forward_mode():
+        return op(*args)
+    with torch.autograd.forward_ad._set_fwd_grad_enabled(False):
+        return op(*args)
+
+
 class _GatedFn(torch.autograd.Function):
     """torch.ops.mst.gated_recurrence's registered backward as one autograd node."""
 
@@ -624,6 +634,7 @@ class _GatedFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_h, g_last):
         x, gate, h0, lengths, carry = ctx.saved_tensors
+        K.refuse_tangents("gated_recurrence_backward", g_h, g_last)
         need = ctx.needs_input_grad[2]
         dx, dgate, dh0 = K.gated_bwd(g_h, g_last, x, gate, h0, lengths, carry, ctx.reverse, need)
         return dx, dgate, dh0.to(h0.dtype) if need else None, None, None
@@ -632,7 +643,8 @@ class _GatedFn(torch.autograd.Function):
 def gated_recurrence_step(x, gate, state):
     """One frame of gated_recurrence for serving: x, gate (B, C); state (B, C) float32 contiguous is
     updated in place and its new values are returned in x's type. Not differentiable."""
+    K.refuse_tangents("gated_recurrence_step", x, gate, state)
     if _eager(x, gate, state) and not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
                                                                     or state.requires_grad)):
         return K.gated_step(x, gate, state)
-    return torch.ops.mst.gated_recurrence_step(x, gate, state)
+    return _op(torch.ops.mst.gated_recurrence_step, x, gate, state)

@@ -18,6 +18,7 @@ import threading
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -518,6 +519,17 @@ def gated_tiles(dtype, T):
     512 frames in float32 and up to 1024 in 16 bits."""
     one = GATED_TILE if dtype == torch.float32 else 2 * GATED_TILE
     return (T + GATED_TILE - 1) // GATED_TILE if T > one else 0
+
+
+def refuse_tangents(what, *ts):
+    """The recurrence has no forward-mode derivative: a tensor that carries a tangent (a dual tensor,
+    torch.func.jvp) is refused, where the kernels would drop the tangent without a word."""
+    if in_forward_mode() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"{what}: no forward-mode derivative (reverse mode only)")
+
+
+def in_forward_mode():
+    return forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
 
 
 def gated_check(x, gate, h0, lengths):

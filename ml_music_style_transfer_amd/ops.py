@@ -517,11 +517,21 @@ def gated_recurrence(x: Tensor, gate: Tensor, h0: Optional[Tensor], lengths: Opt
     """a_t = sigmoid(gate_t), h_t = a_t h_{t-1} + (1 - a_t) x_t over (B, C, T) from h0 (B, C);
     frames at or past lengths[b] leave the state and give 0; reverse: t runs down. Returns h in
     x's type, the final state and the kept states of the backward (B, C, tiles), both float32."""
+    _reverse_mode_only("gated_recurrence")
     return K.gated_fwd(x, gate, h0, lengths, reverse)
+
+
+def _reverse_mode_only(what):
+    """An operator's body sees the tangents of dual tensors but none of torch.func.jvp's, and its output
+    has none: within forward mode it is refused whatever its inputs (engine's functions look at them)."""
+    if K.in_forward_mode():
+        raise NotImplementedError(f"{what}: no forward-mode derivative (reverse mode only); "
+                                  "engine's function takes inputs that carry no tangent")
 
 
 @gated_recurrence.register_fake
 def _gated_fake(x, gate, h0, lengths, reverse):
+    _reverse_mode_only("gated_recurrence")
     K.gated_check(x, gate, h0, lengths)
     B, C, T = x.shape
     return (x.new_empty(B, C, T), x.new_empty(B, C, dtype=torch.float32),
@@ -533,11 +543,13 @@ def gated_recurrence_backward(grad_h: Optional[Tensor], grad_last: Optional[Tens
                               gate: Tensor, h0: Optional[Tensor], lengths: Optional[Tensor],
                               carry: Tensor, reverse: bool) -> Tuple[Tensor, Tensor, Tensor]:
     """(d x, d gate, d h0 in float32) of gated_recurrence."""
+    _reverse_mode_only("gated_recurrence_backward")
     return K.gated_bwd(grad_h, grad_last, x, gate, h0, lengths, carry, reverse)
 
 
 @gated_recurrence_backward.register_fake
 def _gated_bwd_fake(grad_h, grad_last, x, gate, h0, lengths, carry, reverse):
+    _reverse_mode_only("gated_recurrence_backward")
     K.gated_bwd_check(grad_h, grad_last, x, gate, h0, lengths, carry)
     B, C, T = x.shape
     return x.new_empty(B, C, T), x.new_empty(B, C, T), x.new_empty(B, C, dtype=torch.float32)
@@ -563,11 +575,13 @@ gated_recurrence.register_autograd(_gated_backward, setup_context=_gated_setup)
 @custom_op("mst::gated_recurrence_step", mutates_args=("state",))
 def gated_recurrence_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
     """One frame of gated_recurrence: x, gate (B, C); state (B, C) float32, updated in place."""
+    _reverse_mode_only("gated_recurrence_step")
     return K.gated_step(x, gate, state)
 
 
 @gated_recurrence_step.register_fake
 def _gated_step_fake(x, gate, state):
+    _reverse_mode_only("gated_recurrence_step")
     K.gated_step_check(x, gate, state)
     return x.new_empty(x.shape)
 
