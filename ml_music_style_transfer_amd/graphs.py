@@ -165,8 +165,7 @@ class GraphedTrainStep:
                 self._program(st)
             self._captured_st = st
             self.graph.replay()
-        if self.max_norm is not None:
-            self.opt.grad_norm = self.norm
+        self.opt.grad_norm = self.norm if self.max_norm is not None else None
         self.calls += 1
         self.opt._count_step(st, self.params)
         self._host_step = st["step"]

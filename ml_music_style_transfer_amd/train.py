@@ -51,8 +51,8 @@ class Adam(torch.optim.Optimizer):
 
     max_norm: every step takes the gradients times min(1, max_norm / (norm + 1e-6)), norm being
     the L2 norm over all gradients of all groups (clip_grad_norm_'s factor). The factor is applied
-    inside the update: p.grad stays as backward left it, and `grad_norm` is the step's norm (a
-    0-d device tensor; reading it waits for the device).
+    inside the update: p.grad stays as backward left it, and `grad_norm` is the last step's norm (a
+    0-d device tensor; reading it waits for the device; None after a step without a limit).
     """
 
     max_norm = None
@@ -181,6 +181,7 @@ class Adam(torch.optim.Optimizer):
         for owner in _owners(p for group in self.param_groups for p in group["params"]):
             if owner is not attached:
                 dp.finish_gradients(owner)
+        self.grad_norm = None
         bwd = getattr(self, "_bwd", None)
         if bwd is not None and bwd.finish():  # the update already ran inside backward
             self._count_step(bwd.st, bwd.params)
@@ -236,6 +237,7 @@ class Adam(torch.optim.Optimizer):
                 raise TypeError("Adam: float32 parameters and gradients")
             groups.append((group, params, flat, st))
         if not groups:
+            self.grad_norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
             return
         self.grad_norm = K.grad_norm(grads)
         torch.autograd.graph.increment_version([p for _, params, _, _ in groups for p in params])
