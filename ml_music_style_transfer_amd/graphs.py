@@ -152,7 +152,8 @@ class GraphedTrainStep:
             self.lr_dev.fill_(lr)
             self._lr = lr
         if self.opt.max_norm != self.max_norm:  # a constant of the captured update
-            self.max_norm, self.graph = self.opt.max_norm, None
+            limit = self.opt.max_norm
+            self.max_norm, self.graph = None if limit is None else K.check_max_norm(limit), None
         st = self._state()
         self.model.train()
         if self.graph is not None:

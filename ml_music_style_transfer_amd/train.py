@@ -222,6 +222,7 @@ class Adam(torch.optim.Optimizer):
         """step() with a max_norm: the norm over every group's gradients, then each group's update
         (flat buffers: their ranges between the paddings; otherwise lists of tensors, one launch
         sequence for the parameters of one step count)."""
+        max_norm = K.check_max_norm(self.max_norm)  # a limit may be set between steps
         groups, grads = [], []
         for gi, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
@@ -246,8 +247,8 @@ class Adam(torch.optim.Optimizer):
             lr, eps = group["lr"], group["eps"]
 
             def update(tensors, t):
-                K.adam_clip(*zip(*tensors), self.grad_norm, self.max_norm, lr / (1 - b1 ** t), b1, b2,
-                            eps, math.sqrt(1 - b2 ** t))
+                K.adam_clip(*zip(*tensors), self.grad_norm, max_norm, lr / (1 - b1 ** t), b1, b2, eps,
+                            math.sqrt(1 - b2 ** t))
 
             if st is not None:
                 pf, gf, owner = flat

@@ -133,6 +133,20 @@ def test_the_norm_is_the_last_step_s(kernels):
     assert opt.grad_norm is None
 
 
+@pytest.mark.parametrize("bad", [-1.0, float("nan")])
+def test_a_limit_set_later_is_checked(kernels, bad):
+    """and refused before a parameter, a moment or a step count changes."""
+    free = nn.Parameter(torch.zeros(4))
+    free.grad = torch.ones(4)
+    opt = T.Adam([free], max_norm=1.0)
+    opt.step()
+    state = {k: v.clone() for k, v in opt.state[free].items()}
+    opt.max_norm = bad
+    with pytest.raises(ValueError, match="max_norm"):
+        opt.step()
+    assert all(torch.equal(opt.state[free][k], v) for k, v in state.items()) and (free == -1).all()
+
+
 @pytest.mark.gpu
 def test_captured_step_without_its_limit(cuda):
     """A limit taken away between replays: the step after it reports no norm."""
