@@ -245,7 +245,8 @@ int mst_gated_bwd(int32_t type, const void* x, int64_t xb, int64_t xc, const voi
                   const void* gh, const float* glast, int32_t B, int32_t C, int32_t T, int32_t reverse,
                   void* dx, void* dgate, float* dh0, void* workspace, size_t ws_bytes, void* stream);
 /* One frame: state (B, C) is updated in place and h (B, C) contiguous receives it; x, gate (B, C)
- * by batch stride, unit channel stride. */
+ * by batch stride, unit channel stride. What is written lies apart from what is read, or is it element
+ * for element (MST_EINVAL otherwise). */
 int mst_gated_step(int32_t type, const void* x, int64_t xb, const void* gate, int64_t gb, int32_t B,
                    int32_t C, float* state, void* h, void* stream);
 

@@ -626,6 +626,22 @@ bool good_shape(int32_t type, int32_t B, int32_t C, int32_t T) {
          (long long)B * C < (1ll << 31) && (long long)B * C * lanes_of(T) < (1ll << 32) - 256;
 }
 
+// Whether C values of `z` bytes in each of B rows at `p` lie apart from the B C contiguous values of `wz`
+// bytes that are written at `w`, or are these themselves (a thread then reads what it alone writes).
+bool apart(const void* p, int64_t stride, int z, const void* w, int wz, int32_t B, int32_t C) {
+  if (p == w && z == wz && (B == 1 || stride == C)) return true;
+  const __int128 row = (__int128)C * z, s = (uintptr_t)w, e = s + (__int128)B * C * wz;
+  __int128 a = (uintptr_t)p, step = (__int128)stride * z;
+  if (step < 0) a += step * (B - 1), step = -step;
+  if (a + row <= s) {  // the first row that ends behind the start of w
+    if (step == 0) return true;
+    const __int128 k = (s - row - a) / step + 1;
+    if (k >= B) return true;
+    a += k * step;
+  }
+  return a >= e;
+}
+
 }  // namespace
 
 extern "C" {
@@ -672,6 +688,10 @@ int mst_gated_bwd(int32_t type, const void* x, int64_t xb, int64_t xc, const voi
 int mst_gated_step(int32_t type, const void* x, int64_t xb, const void* gate, int64_t gb, int32_t B,
                    int32_t C, float* state, void* h, void* stream) {
   MST_REQUIRE(good_shape(type, B, C, 1) && x && gate && state && h);
+  const int z = type == MST_F32 ? 4 : 2;
+  MST_REQUIRE(apart(x, xb, z, state, 4, B, C) && apart(gate, gb, z, state, 4, B, C));
+  MST_REQUIRE(apart(x, xb, z, h, z, B, C) && apart(gate, gb, z, h, z, B, C));
+  MST_REQUIRE(apart(h, C, z, state, 4, B, C));
   const long long n = (long long)B * C;
   const dim3 grid((unsigned)((n + 255) / 256));
   hipStream_t st = (hipStream_t)stream;

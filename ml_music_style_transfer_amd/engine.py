@@ -642,7 +642,8 @@ class _GatedFn(torch.autograd.Function):
 
 def gated_recurrence_step(x, gate, state):
     """One frame of gated_recurrence for serving: x, gate (B, C); state (B, C) float32 contiguous is
-    updated in place and its new values are returned in x's type. Not differentiable."""
+    updated in place and its new values are returned in x's type; x and gate lie outside its memory (x may
+    be the state itself). Not differentiable."""
     K.refuse_tangents("gated_recurrence_step", x, gate, state)
     if _eager(x, gate, state) and not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
                                                                     or state.requires_grad)):

@@ -664,7 +664,7 @@ def gated_step(x, gate, state):
         with L.device_of(x.device):
             L.check(_lib().mst_gated_step(L.TYPES[x.dtype], _p(x), x.stride(0), _p(gate),
                                           gate.stride(0), B, C, _p(state), _p(h), L.stream()),
-                    "gated_recurrence_step")
+                    "gated_recurrence_step (x or gate in the state's memory?)")
         torch.autograd.graph.increment_version(state)
     return h
 
