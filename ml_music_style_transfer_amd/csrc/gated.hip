@@ -147,12 +147,18 @@ __device__ __forceinline__ void store(T* row, int t, int end, const float (&v)[V
 // a = sigmoid(g) and c = 1 - a, each to its own relative precision (c is not formed from a).
 // e^-|g| = 2^t e^(-|g| - t ln 2) with t = -|g| log2(e) rounded: the second factor is 1 + a rounding's
 // size (taken into [-1, 1], since an infinite g makes its exponent no number where 2^t is zero; of a
-// g that is no number 2^t is none either). The quotient is the hardware's, to its last place.
+// g that is no number 2^t is none either). e keeps the hardware exponential's error of one place and its
+// correction's half (worst measured: 4.4 x 2^-24 of e). The quotient is the hardware's, to its last place,
+// and for float32 tensors brought to the nearest by a step of Newton's: a on gates of 3 to 16 is off by
+// 1.50 x 2^-24 at worst, 1.82 without; (32, 1024, 252) takes 17.2 + 27.2 us, 17.1 + 27.1 without. 16-bit
+// kernels have no instruction to spare, and round what they store to 2^-8 or 2^-11.
+template <typename T>
 __device__ __forceinline__ void gate_of(float g, float& a, float& c) {
   const float t = fabsf(g) * -1.44269504f;
   float e = __builtin_amdgcn_exp2f(t);
   e = fmaf(e, __builtin_amdgcn_fmed3f(fmaf(t, -0.693147181f, -fabsf(g)), -1.f, 1.f), e);
-  const float r = __builtin_amdgcn_rcpf(1.f + e);
+  float r = __builtin_amdgcn_rcpf(1.f + e);
+  if constexpr (sizeof(T) == 4) r = fmaf(fmaf(-(1.f + e), r, 1.f), r, r);
   const float er = e * r;
   a = g < 0.f ? er : r;
   c = g < 0.f ? r : er;
@@ -356,7 +362,7 @@ __global__ __launch_bounds__(256) void gated_maps_kernel(const Args p) {
 #pragma unroll
     for (int q = 0; q < V; ++q) {
       const int k = DOWN ? V - 1 - q : q;
-      gate_of(g[k], a[k], c[k]);
+      gate_of<T>(g[k], a[k], c[k]);
       H = BWD ? a[k] * (b[k] + H) : fmaf(a[k], H, c[k] * b[k]);
       A *= a[k];
     }
@@ -418,7 +424,7 @@ __global__ __launch_bounds__(256) void gated_fwd_kernel(const Args p) {
 #pragma unroll
     for (int q = 0; q < V; ++q) {
       const int k = REV ? V - 1 - q : q;
-      gate_of(g[k], a[k], c[k]);
+      gate_of<T>(g[k], a[k], c[k]);
       b[k] *= c[k];
       H = fmaf(a[k], H, b[k]);
       A *= a[k];
@@ -492,7 +498,7 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(const Args p) {
       clear(r.len - now, d);
     }
 #pragma unroll
-    for (int k = 0; k < V; ++k) gate_of(g[k], a[k], c[k]);
+    for (int k = 0; k < V; ++k) gate_of<T>(g[k], a[k], c[k]);
     float A = 1.f, H = 0.f, U = 0.f, At, Ht;
 #pragma unroll
     for (int q = 0; q < V; ++q) {
@@ -547,7 +553,7 @@ __global__ __launch_bounds__(256) void gated_step_kernel(const T* __restrict__ x
   if (i >= n) return;
   const long long b = i / C, c = i % C;
   float a, cc;
-  gate_of((float)gate[b * gb + c], a, cc);
+  gate_of<T>((float)gate[b * gb + c], a, cc);
   const float s = fmaf(a, state[i], cc * (float)x[b * xb + c]);
   state[i] = s;
   h[i] = (T)s;

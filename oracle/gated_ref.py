@@ -3,8 +3,10 @@ on what a float32 evaluation of the same formulas, in any order of composition, 
 
   a_t = sigmoid(gate_t), c_t = 1 - a_t, h_t = a_t h_{t-1} + c_t x_t; frames t >= length are the identity
 
-Error model, u = 2^-24 (half a float32 step): an exponential within 4u, 1 + e, the quotient and e r one
-rounding each give a and c to 9u; c x to 10u. A state of magnitude M (the recurrence run on |x|, |h0|)
+Error model, u = 2^-24 (half a float32 step): e = e^-|gate| within 3u + |gate| u / 20 (an exponential and its
+correction, ln 2 in float32), 7.4u before it underflows; 1 + e one rounding, a quotient r within 2u (exact
+where e < u), e r one rounding. r passes on at most half of e's error (|gate| near 0), so r is within 4.5u,
+e r within 8.5u: a and c to 9u; c x to 10u. A state of magnitude M (the recurrence run on |x|, |h0|)
 that passes a frame gains at most a's 9u and two roundings, 11u a M in all; the frame's own term its 10u
 and the sum's rounding; composing maps in a tree rounds a term at most once a level, and a term has
 passed at least as many frames as levels. With M_t = a_t M_{t-1} + c_t |x_t| both are within
