@@ -639,12 +639,8 @@ bool apart(const void* p, int64_t stride, int z, const void* w, int wz, int32_t 
   const __int128 row = (__int128)C * z, s = (uintptr_t)w, e = s + (__int128)B * C * wz;
   __int128 a = (uintptr_t)p, step = (__int128)stride * z;
   if (step < 0) a += step * (B - 1), step = -step;
-  if (a + row <= s) {  // the first row that ends behind the start of w
-    if (step == 0) return true;
-    const __int128 k = (s - row - a) / step + 1;
-    if (k >= B) return true;
-    a += k * step;
-  }
+  if (a >= e || a + step * (B - 1) + row <= s) return true;
+  if (a + row <= s) a += ((s - row - a) / step + 1) * step;  // the first row that ends behind the start of w
   return a >= e;
 }
 

@@ -26,6 +26,7 @@ Gradient accumulation follows torch semantics: a parameter whose .grad is None
 gets a fresh gradient (written, not added); otherwise the kernel adds into it.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import kernels as K
@@ -590,9 +591,8 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
 
     Returns (h, last): h (B, C, T) in x's type, last (B, C) float32, the state that the next chunk
     starts from. Differentiable in x, gate and h0, in reverse mode, once; states are float32 inside."""
-    K.refuse_tangents("gated_recurrence", x, gate, h0)
     if not _eager(x, gate, h0):
-        h, last, _ = _op(torch.ops.mst.gated_recurrence, x, gate, h0, lengths, bool(reverse))
+        h, last, _ = _ops.without_tangents(torch.ops.mst.gated_recurrence, x, gate, h0, lengths, bool(reverse))
     elif torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
                                       or (h0 is not None and h0.requires_grad)):
         h, last = _GatedFn.apply(x, gate, h0, lengths, bool(reverse))
@@ -605,18 +605,9 @@ def _eager(*ts):
     """True for ordinary tensors that nothing traces or transforms: the kernels may then be called
     without the dispatcher's layers, which cost more than a small call's kernel (a single frame of
     1025 channels: 17.5 us a call through them, 9.6 without, its kernel 2)."""
-    return (not torch.compiler.is_compiling() and not torch.jit.is_tracing()
+    return (not torch.compiler.is_compiling() and not torch._C._is_tracing() and forward_ad._current_level < 0
             and torch._C._len_torch_dispatch_stack() == 0 and torch._C._functorch.peek_interpreter_stack() is None
             and all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts))
-
-
-def _op(op, *args):
-    """The registered operator on inputs without tangents. Inside forward mode it cannot tell (it sees
-    none of torch.func.jvp's tangents) and refuses, unless forward mode is off around it."""
-    if not K.in_forward_mode():
-        return op(*args)
-    with torch.autograd.forward_ad._set_fwd_grad_enabled(False):
-        return op(*args)
 
 
 class _GatedFn(torch.autograd.Function):
@@ -644,8 +635,7 @@ def gated_recurrence_step(x, gate, state):
     """One frame of gated_recurrence for serving: x, gate (B, C); state (B, C) float32 contiguous is
     updated in place and its new values are returned in x's type; x and gate lie outside its memory (x may
     be the state itself). Not differentiable."""
-    K.refuse_tangents("gated_recurrence_step", x, gate, state)
     if _eager(x, gate, state) and not (torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
                                                                     or state.requires_grad)):
         return K.gated_step(x, gate, state)
-    return _op(torch.ops.mst.gated_recurrence_step, x, gate, state)
+    return _ops.without_tangents(torch.ops.mst.gated_recurrence_step, x, gate, state)

@@ -29,6 +29,7 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.library import custom_op
 
 from . import _lib as L
@@ -529,6 +530,16 @@ def _reverse_mode_only(what):
                                   "engine's function takes inputs that carry no tangent")
 
 
+def without_tangents(op, *args):
+    """`op` on arguments that are known to carry no tangent: with forward mode off around it, its body
+    does not refuse them."""
+    if not K.in_forward_mode():
+        return op(*args)
+    K.refuse_tangents(op.__name__, *(t for t in args if isinstance(t, Tensor) and t.is_floating_point()))
+    with forward_ad._set_fwd_grad_enabled(False):
+        return op(*args)
+
+
 @gated_recurrence.register_fake
 def _gated_fake(x, gate, h0, lengths, reverse):
     _reverse_mode_only("gated_recurrence")
@@ -564,8 +575,8 @@ def _gated_setup(ctx, inputs, output):
 
 def _gated_backward(ctx, g_h, g_last, g_carry):
     x, gate, h0, lengths, carry = ctx.saved_tensors
-    dx, dgate, dh0 = torch.ops.mst.gated_recurrence_backward(g_h, g_last, x, gate, h0, lengths, carry,
-                                                             ctx.reverse)
+    dx, dgate, dh0 = without_tangents(torch.ops.mst.gated_recurrence_backward, g_h, g_last, x, gate, h0, lengths,
+                                      carry, ctx.reverse)
     return dx, dgate, dh0.to(h0.dtype) if h0 is not None else None, None, None
 
 

@@ -149,9 +149,10 @@ def test_a_limit_set_later_is_checked(kernels, bad):
 
 @pytest.mark.gpu
 def test_captured_step_without_its_limit(cuda):
-    """A limit taken away between replays: the step after it reports no norm."""
+    """A limit taken away between replays: the step after it reports no norm. The optimizer finds the
+    model through its parameters."""
     net = PerformanceNet().to(cuda).train()
-    opt = T.make_optimizer(net, max_norm=0.01)
+    opt = T.Adam(net.parameters(), max_norm=0.01)
     step = GraphedTrainStep(net, opt, warmup=1)
     data = [torch.from_numpy(a).to(cuda) for a in detinit.model_inputs(1, 44)]
     for _ in range(3):
