@@ -605,9 +605,13 @@ def _eager(*ts):
     """True for ordinary tensors that nothing traces or transforms: the kernels may then be called
     without the dispatcher's layers, which cost more than a small call's kernel (a single frame of
     1025 channels: 17.5 us a call through them, 9.6 without, its kernel 2)."""
-    return (not torch.compiler.is_compiling() and not torch._C._is_tracing() and forward_ad._current_level < 0
-            and torch._C._len_torch_dispatch_stack() == 0 and torch._C._functorch.peek_interpreter_stack() is None
-            and all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in ts))
+    if (torch.compiler.is_compiling() or torch._C._is_tracing() or forward_ad._current_level >= 0
+            or torch._C._len_torch_dispatch_stack() or torch._C._functorch.peek_interpreter_stack() is not None):
+        return False
+    for t in ts:
+        if t is not None and type(t) not in (torch.Tensor, torch.nn.Parameter):
+            return False
+    return True
 
 
 class _GatedFn(torch.autograd.Function):

@@ -178,9 +178,10 @@ class Adam(torch.optim.Optimizer):
         attached = getattr(self, "_owner", None)
         if attached is not None:
             dp.finish_gradients(attached)  # overlapped data-parallel all-reduces must land first
-        for owner in _owners(p for group in self.param_groups for p in group["params"]):
-            if owner is not attached:
-                dp.finish_gradients(owner)
+        if dp.is_dist():
+            for group in self.param_groups:
+                for owner in _owners(group["params"]):
+                    dp.finish_gradients(owner)
         self.grad_norm = None
         bwd = getattr(self, "_bwd", None)
         if bwd is not None and bwd.finish():  # the update already ran inside backward
@@ -281,8 +282,14 @@ _memory_order = K.memory_order
 
 def _owners(params):
     """The models whose flat buffers the parameters live in, in the parameters' order."""
-    refs = {id(ref): ref for ref in (getattr(p, "_mst_flat_owner", None) for p in params) if ref is not None}
-    return [owner for owner in (ref() for ref in refs.values()) if owner is not None]
+    owners, last = [], None
+    for p in params:
+        ref = getattr(p, "_mst_flat_owner", None)
+        if ref is not last:
+            last, owner = ref, ref() if ref is not None else None
+            if owner is not None and owner not in owners:
+                owners.append(owner)
+    return owners
 
 
 def _grads_of(parameters, what):
