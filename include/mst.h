@@ -208,15 +208,15 @@ int mst_adam_dev_f32(float* p, const float* g, float* m, float* v, int64_t n, co
  * tensor's memory); grads, numel and types are HOST arrays, read before the call returns.
  *   norm[0] = sqrt(sum of g^2 over every element)  (sums in double, in one fixed order)
  * scale: g *= min(1, max_norm / (norm[0] + 1e-6)) in place (max_norm >= 0), the product in float,
- * rounded once to the element type. A norm that is not a number makes the factor one. Ranges that
- * are written must not overlap (MST_EINVAL). */
+ * rounded once to the element type. A NaN norm makes the factor NaN, and every value that is scaled;
+ * an infinite one makes it 0. Ranges that are written must not overlap (MST_EINVAL). */
 size_t mst_grad_norm_workspace_size(int32_t count);
 int mst_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* types, int32_t count,
                   float* norm, void* workspace, size_t ws_bytes, void* stream);
 int mst_grad_scale(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count,
                    const float* norm, float max_norm, void* stream);
 /* mst_adam_f32's update over `count` tensors (HOST arrays of device pointers), each gradient taken
- * times min(1, max_norm / (norm[0] + 1e-6)); the gradients stay as they are. hyper (nullable) as in
+ * times min(1, max_norm / (norm[0] + 1e-6)) (NaN norms as above); the gradients stay as they are. hyper (nullable) as in
  * mst_adam_dev_f32. The elements of p, g, m, v of one tensor are in one order; 4-byte alignment. */
 int mst_adam_clip_f32(float* const* p, const float* const* g, float* const* m, float* const* v,
                       const int64_t* numel, int32_t count, const float* norm, float max_norm,
@@ -231,7 +231,7 @@ int mst_adam_clip_f32(float* const* p, const float* const* g, float* const* m, f
  * h: (B, C, T) contiguous; last (B, C): the state after the last frame (the first when reversed).
  * carry: B * C * mst_gated_tiles(type, T) floats for the backward (nullable when that is 0); workspace
  * of mst_gated_workspace_size bytes (nullable when that is 0), for _fwd and _bwd alike. States are
- * float whatever the type. */
+ * float whatever the type. What is written overlaps nothing that is read. */
 int32_t mst_gated_tiles(int32_t type, int32_t T);
 size_t mst_gated_workspace_size(int32_t type, int32_t B, int32_t C, int32_t T);
 int mst_gated_fwd(int32_t type, const void* x, int64_t xb, int64_t xc, const void* gate, int64_t gb,

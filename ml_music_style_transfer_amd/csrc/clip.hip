@@ -7,9 +7,9 @@
 // captured graph keeps them). Each tensor is cut into chunks; workgroup k takes the launch's chunks
 // k, k + gridDim.x, ... All of it is bound by HBM. Small chunks in order keep what is in flight close
 // together in memory: over 726 M parameters, chunks of 16384 / 4096 / 1024 elements run the norm in
-// 472 / 459 / 555 us (a lookup a chunk; 6.3 TB/s) and Adam in 3.81 / 3.50 / 3.37 ms (6.0 TB/s; its
-// predecessor without the clip 4.11 ms on the same card; without nontemporal access 3.96 -> 3.77 at
-// most).
+// 472 / 459 / 555 us (a lookup a chunk; 6.3 TB/s) and Adam in 3.81 / 3.50 / 3.37 ms (ten calls in a row, 6.0
+// TB/s; its predecessor without the clip 4.11 ms on the same card; without nontemporal access 3.96 -> 3.77
+// at most). Traced between other kernels Adam's median is 3.43 to 3.58 ms, 5.7 to 5.9 TB/s.
 #include <new>
 
 #include "common.h"

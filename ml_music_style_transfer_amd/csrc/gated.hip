@@ -19,10 +19,11 @@
 //
 // Bound by HBM in float32: (32, 1024, 252) takes 17 us forward and 27 us backward, 5.9 and 6.2 TB/s
 // of the 3 and 5 tensors that have to move. In 16 bits also by the vector unit's issue: a frame
-// costs some 28 instructions forward and 43 backward (14 of them its gate), and (16, 4096, 860) in
-// bfloat16 runs at 5.5 and 5.3 TB/s with 93 % and 84 % of the issue slots taken. Rows of an odd
-// number of 16-bit frames, which start off any alignment, are the slowest ((64, 8192, 63) backward 84 us,
-// 3.9 TB/s).
+// costs some 28 instructions forward and 43 backward (14 of them its gate; two more in float32), and
+// (16, 4096, 860) in bfloat16 takes 62 and 107 us, 5.5 and 5.3 TB/s. With padded clips, whose loads stop at
+// their lengths but whose frames are all computed, it takes nearly as long (61 and 101 us; 93 % and 84 % of the
+// issue slots, 3.8 and 4.0 TB/s of what has to move): issue alone. Rows of an odd number of 16-bit
+// frames, which start off any alignment, are the slowest ((64, 8192, 63) backward 83 us, 4.0 TB/s).
 #include "common.h"
 
 namespace {
@@ -575,7 +576,10 @@ int tiles_of(int32_t type, int32_t T) {
 // read x and gate (gate and gh) twice and cost a launch. Float32, forward + backward, one wave a row
 // -> segments: 128 rows of 50001 frames 76 + 104 -> 27 + 36 us, 512 of 60000 110 + 219 -> 109 + 176, but
 // 1024 of 8192 (16 tiles) 20 + 30 -> 31 + 43 and 300 of 3500 (7 tiles) 16 + 17 -> 22 + 23. 8192 waves fill
-// the chip's slots (2048 waves: 117 + 197 in the second case).
+// the chip's slots (2048 waves: 117 + 197 in the second case). Both bounds lie between those points and are
+// not measured close by, nor in 16 bits: few rows of 8 to 19 tiles may be better cut. A segment's last turn
+// fetches its neighbour's first tile and drops it (in range, but read for nothing: at two tiles a segment
+// the three kernels read 60, 69 and 106 MB where 51, 51 and 77 would do).
 int span_of(long long rows, int tiles) {
   if (rows > 640 || tiles < 20) return tiles;
   return (int)((rows * tiles + 8191) / 8192);

@@ -586,8 +586,9 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
     from the last frame to the first. lengths (B,): frames at or past a clip's length are not used,
     give h = 0 and no gradient, and leave the state as it is.
 
-    A value or gate that is not finite makes the row's state that from its frame on; no frame before
-    it and no other row is touched.
+    A value or gate that is NaN makes the row's states NaN from its frame on, an infinite value (or h0)
+    makes them infinite or NaN (a state that decays to 0 times infinity); a gate of +inf holds the state
+    and one of -inf replaces it by x, exactly. No frame before it and no other row is touched.
 
     Returns (h, last): h (B, C, T) in x's type, last (B, C) float32, the state that the next chunk
     starts from. Differentiable in x, gate and h0, in reverse mode, once; states are float32 inside."""
@@ -602,7 +603,8 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
 
 
 def _eager(*ts):
-    """True for ordinary tensors that nothing traces or transforms: the kernels may then be called
+    """True for ordinary tensors that nothing traces or transforms (no compiler, torch.jit.trace, forward
+    mode, dispatch mode or torch.func): the kernels may then be called
     without the dispatcher's layers, which cost more than a small call's kernel (a single frame of
     1025 channels: 17.5 us a call through them, 9.6 without, its kernel 2)."""
     if (torch.compiler.is_compiling() or torch._C._is_tracing() or forward_ad._current_level >= 0
