@@ -231,12 +231,10 @@ class Adam(torch.optim.Optimizer):
                 continue
             flat = self._flat_of(group, params)
             st = self._flat_state(gi, flat[0], params) if flat is not None else None
-            if st is not None:
-                grads += [flat[1][o:o + n] for o, n in flat[2].flat_runs()]
-            else:
-                grads += [p.grad for p in params]
-            if any(t.dtype != torch.float32 for p in params for t in (p, p.grad)):
+            own = [p.grad for p in params]
+            if {t.dtype for t in params} != {torch.float32} or {t.dtype for t in own} != {torch.float32}:
                 raise TypeError("Adam: float32 parameters and gradients")
+            grads += own if st is None else [flat[1][o:o + n] for o, n in flat[2].flat_runs()]
             groups.append((group, params, flat, st))
         if not groups:
             self.grad_norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
