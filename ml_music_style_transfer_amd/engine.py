@@ -604,9 +604,9 @@ def gated_recurrence(x, gate, h0=None, lengths=None, reverse=False):
 
 def _eager(*ts):
     """True for ordinary tensors that nothing traces or transforms (no compiler, torch.jit.trace, forward
-    mode, dispatch mode or torch.func): the kernels may then be called
-    without the dispatcher's layers, which cost more than a small call's kernel (a single frame of
-    1025 channels: 17.5 us a call through them, 9.6 without, its kernel 2)."""
+    mode, dispatch mode or torch.func): the kernels may then be called without the dispatcher's layers,
+    which cost more than a small call's kernel (a single frame of 1025 channels: 17.5 us a call through
+    them, 9.6 without, its kernel 2)."""
     if (torch.compiler.is_compiling() or torch._C._is_tracing() or forward_ad._current_level >= 0
             or torch._C._len_torch_dispatch_stack() or torch._C._functorch.peek_interpreter_stack() is not None):
         return False

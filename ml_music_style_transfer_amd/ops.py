@@ -531,8 +531,8 @@ def _reverse_mode_only(what):
 
 
 def without_tangents(op, *args):
-    """`op` on arguments that are known to carry no tangent: with forward mode off around it, its body
-    does not refuse them."""
+    """`op` on arguments that carry no tangent (refused otherwise): with forward mode off around it, its
+    body does not refuse them."""
     if not K.in_forward_mode():
         return op(*args)
     K.refuse_tangents(op.__name__, *(t for t in args if isinstance(t, Tensor) and t.is_floating_point()))
